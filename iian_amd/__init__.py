@@ -9,6 +9,9 @@ from .paged_attn import (  # noqa: F401
     GGML_TYPE_F16,
     GGML_TYPE_F32,
     GGML_TYPE_Q8_0,
+    MROPE_INTERLEAVED,
+    MROPE_RESTART,
+    MROPE_SECTIONS,
     KVPool,
     PagedAttnParams,
     PagedAttnRuntime,
@@ -16,15 +19,22 @@ from .paged_attn import (  # noqa: F401
     RequestBlocks,
     RopeParams,
     bind_build_batch,
+    bind_mrope_positions,
+    bind_mrope_set_rows_kv,
     bind_paged_attn,
+    bind_prompt_attn,
     bind_rope_set_rows_kv,
     bind_set_rows_kv,
     bind_write_paged_attn,
     build_batch,
     build_paged_attn,
     dequant_q8_0,
+    mrope_frequencies,
+    mrope_positions,
+    mrope_set_rows_kv,
     new_workspace,
     paged_attn_supported,
+    prompt_attn,
     rope_set_rows_kv,
     row_bytes,
     set_rows,

@@ -22,6 +22,11 @@ NOALLOC_SCRATCH_BYTES = 64 << 20
 TYPE_F32 = 0
 TYPE_F16 = 1
 TYPE_Q8_0 = 8
+TYPE_BF16 = 30
+
+MROPE_SECTIONS = 0
+MROPE_INTERLEAVED = 1
+MROPE_RESTART = 2
 
 # name -> (restype, argtypes); exactly the entry points of include/iian_pa.h
 _P = C.c_void_p
@@ -46,6 +51,12 @@ SIGNATURES = {
     "iian_pa_swa_free_blocks": (C.c_int, [_P, _P, _P, _I32, _I32, _I32, _I32, _P, _P, _I32]),
     "iian_pa_rope_kv_write": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _I64,
                                         C.c_int, C.c_int, _P]),
+    "iian_pa_mrope_positions": (C.c_int, [_P, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _P, _P, _P]),
+    "iian_pa_mrope_frequencies": (C.c_int, [_P, _P, _P, _P, _P]),
+    "iian_pa_mrope_kv_write": (C.c_int, [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _I32, _I32,
+                                         C.c_float, _P, _P, _I64, C.c_int, C.c_int, _P]),
+    "iian_pa_prompt_attention": (C.c_int, [_P, _P, _P, _P, C.c_int, _I64, _I64, _I64, _P, _P, _I32, _I32, _I32, _I32,
+                                           _I32, _I32, _I32, C.c_float, C.c_float, _I32, _I32, _P, _I64, _P]),
     "iian_pa_runtime_create": (C.c_int, [_P, _P]),
     "iian_pa_runtime_destroy": (None, [_P]),
     "iian_pa_runtime_begin_step": (C.c_int, [_P, _P, _P, _P, _P, _P, _I32]),
@@ -68,6 +79,19 @@ class RopeParams(C.Structure):
                 ("freq_base", C.c_float), ("freq_scale", C.c_float), ("ext_factor", C.c_float),
                 ("attn_factor", C.c_float), ("beta_fast", C.c_float), ("beta_slow", C.c_float),
                 ("freq_factors", C.c_void_p)]
+
+
+class MRopeAxes(C.Structure):
+    """iian_pa_mrope_axes of include/iian_pa.h."""
+    _fields_ = [("n_axes", C.c_int32), ("layout", C.c_int32), ("sections", C.c_int32 * 4)]
+
+
+class MRopeRows(C.Structure):
+    """iian_pa_mrope_rows of include/iian_pa.h."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_out")] + \
+               [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")] + \
+               [("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("norm_eps", C.c_float), ("type", C.c_int32)]
+
 
 _lib = None
 

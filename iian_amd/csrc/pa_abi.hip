@@ -58,6 +58,7 @@ constexpr int kQ8DecodeWavesPerCu = 8;
 constexpr int kMaxWavesPerCu = kQ8DecodeWavesPerCu;
 constexpr int kDefaultCus = 256;   // an MI355X, when the device cannot be queried
 constexpr int kMaxHeadDim = 1024;  // largest head size the general kernel stages (pa_general.hip)
+constexpr int kMaxPromptTokens = 1 << 30;   // iian_pa_prompt_attention counts tokens and tiles past them in 32 bits
 constexpr int kMaxDevices = 64;
 
 // Compute units of device `dev`, queried once per device.
@@ -275,6 +276,12 @@ size_t split_o_bytes(size_t out_rows, int64_t ns, int head_dim_v) {
 }
 size_t split_bytes(size_t out_rows, int64_t ns, int head_dim_v) {
     return split_o_bytes(out_rows, ns, head_dim_v) + out_rows * (size_t) ns * 2 * sizeof(float);
+}
+
+// Bytes of an element of the rows iian_pa_mrope_kv_write and
+// iian_pa_prompt_attention take, 0 for other types.
+int row_type_bytes(int type) {
+    return type == IIAN_PA_TYPE_F32 ? 4 : type == IIAN_PA_TYPE_F16 || type == IIAN_PA_TYPE_BF16 ? 2 : 0;
 }
 
 // Any head size the general kernel stages (1 .. 1024; the reference's op
@@ -885,6 +892,219 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
     if (rope->ext_factor != 0.0f) p.mscale *= 1.0f + 0.1f * logf(1.0f / rope->freq_scale);
     const hipError_t e = launch_rope_kv_write(p, type_k, type_v, (hipStream_t) stream);
     return e == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
+}
+
+int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
+                            const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
+                            int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag) {
+    if (n_seqs < 0 || n_tokens < 0 || n_spans < 0) return IIAN_PA_ERR_ARG;
+    if (n_seqs == 0 || n_tokens == 0) return IIAN_PA_OK;
+    if ((n_spans > 0 && !spans) || !span_off || !num_computed || !query_start_loc || !pos) return IIAN_PA_ERR_NULL;
+    if ((uintptr_t) spans & 15) return IIAN_PA_ERR_ARG;   // a run is one 16-byte load
+    MropePosParams p = {};
+    p.spans = (const int4 *) spans;
+    p.span_off = span_off;
+    p.num_computed = num_computed;
+    p.qsl = query_start_loc;
+    p.pos = pos;
+    p.row_end = row_end;
+    p.err = err_flag;
+    p.n_spans = n_spans;
+    p.S = n_seqs;
+    p.T = n_tokens;
+    p.grid_full = grid_full ? 1 : 0;
+    return launch_mrope_positions(p, (hipStream_t) stream) == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
+}
+
+int iian_pa_mrope_frequencies(const iian_pa_rope_params *rope, const iian_pa_mrope_axes *axes, double *freqs,
+                              int32_t *axis, float *mscale) {
+    if (!rope || !axes || !freqs || !axis) return IIAN_PA_ERR_NULL;
+    const int n = rope->n_dims, half = n / 2;
+    if (n <= 0 || n % 2 || n > kMaxHeadDim || !(rope->freq_base > 0.0f) || !(rope->freq_scale > 0.0f) ||
+        !std::isfinite(rope->freq_base) || !std::isfinite(rope->freq_scale) || !std::isfinite(rope->ext_factor) ||
+        !std::isfinite(rope->attn_factor))
+        return IIAN_PA_ERR_ARG;
+    if (axes->n_axes < 1 || axes->n_axes > 4 || axes->layout < IIAN_PA_MROPE_SECTIONS ||
+        axes->layout > IIAN_PA_MROPE_RESTART)
+        return IIAN_PA_ERR_ARG;
+    int64_t sum = 0;
+    for (int a = 0; a < axes->n_axes; a++) {
+        if (axes->sections[a] < 0) return IIAN_PA_ERR_ARG;
+        sum += axes->sections[a];
+    }
+    if (sum != half) return IIAN_PA_ERR_ARG;
+    const bool yarn = rope->ext_factor != 0.0f, restart = axes->layout == IIAN_PA_MROPE_RESTART;
+    if (yarn && restart) return IIAN_PA_ERR_UNSUPPORTED;
+    if (yarn && (rope->n_ctx_orig <= 0 || !(rope->beta_fast > 0.0f) || !(rope->beta_slow > 0.0f) ||
+                 rope->freq_base == 1.0f))
+        return IIAN_PA_ERR_ARG;
+    // the YaRN ramp's ends, as iian_pa_rope_kv_write has them, in 64 bits
+    double low = 0, high = 0;
+    if (yarn) {
+        const double k = n / (2 * std::log((double) rope->freq_base));
+        low = std::max(0.0, std::floor(k * std::log(rope->n_ctx_orig / (rope->beta_fast * 2 * M_PI))));
+        high = std::min(n - 1.0, std::ceil(k * std::log(rope->n_ctx_orig / (rope->beta_slow * 2 * M_PI))));
+    }
+    int at = 0, first = 0;   // SECTIONS, RESTART: the section of pair j and its first pair
+    for (int j = 0; j < half; j++) {
+        int a;
+        if (axes->layout == IIAN_PA_MROPE_INTERLEAVED) {
+            const int turn = j % axes->n_axes;
+            a = j < (int64_t) axes->n_axes * axes->sections[turn] ? turn : 0;
+        } else {
+            while (j >= first + axes->sections[at]) first += axes->sections[at++];
+            a = at;
+        }
+        const double e = restart ? (double) (j - first) / axes->sections[at] : 2.0 * j / n;
+        double f = std::pow((double) rope->freq_base, -e) / (rope->freq_factors ? rope->freq_factors[j] : 1.0);
+        if (yarn) {
+            const double ramp = 1.0 - std::min(1.0, std::max(0.0, (j - low) / std::max(0.001, high - low)));
+            const double mix = ramp * rope->ext_factor;
+            f *= rope->freq_scale * (1.0 - mix) + mix;
+        } else {
+            f *= rope->freq_scale;
+        }
+        freqs[j] = f;
+        axis[j] = a;
+    }
+    if (mscale)
+        *mscale = yarn ? (float) (rope->attn_factor * (1.0 + 0.1 * std::log(1.0 / rope->freq_scale)))
+                       : rope->attn_factor;
+    return IIAN_PA_OK;
+}
+
+int iian_pa_mrope_kv_write(void *stream, const iian_pa_mrope_rows *rows, const int32_t *pos, const int64_t *slots,
+                           int64_t n_rows, int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v,
+                           const double *freqs, const int32_t *axis, int32_t n_axes, int32_t n_dims, int32_t mode,
+                           float mscale, void *k_pool, void *v_pool, int64_t n_cells, int type_k, int type_v,
+                           int32_t *err_flag) {
+    if (n_rows < 0 || n_rows > INT32_MAX || n_cells < 0 || n_head < 0 || n_head_kv <= 0 || head_dim <= 0 ||
+        head_dim_v <= 0)
+        return IIAN_PA_ERR_ARG;
+    if (!rows) return IIAN_PA_ERR_NULL;
+    if (n_rows == 0) return IIAN_PA_OK;
+    const iian_pa_mrope_rows &r = *rows;
+    const bool pools = k_pool || v_pool || slots;
+    if (!r.k || !pos || !freqs || !axis) return IIAN_PA_ERR_NULL;
+    if (pools ? !k_pool || !v_pool || !slots || !r.v : !r.k_out) return IIAN_PA_ERR_NULL;
+    if ((r.q == nullptr) != (r.q_out == nullptr) || (r.q && n_head <= 0)) return IIAN_PA_ERR_ARG;
+    if (mode != 0 && mode != 2) return IIAN_PA_ERR_UNSUPPORTED;
+    if (head_dim > kMaxHeadDim || head_dim_v > kMaxHeadDim) return IIAN_PA_ERR_UNSUPPORTED;
+    if (n_axes < 1 || n_axes > 4 || n_dims <= 0 || n_dims % 2 || n_dims > head_dim || !std::isfinite(mscale) ||
+        !(r.norm_eps >= 0.0f) || !std::isfinite(r.norm_eps))
+        return IIAN_PA_ERR_ARG;
+    if (((int64_t) n_head + 2 * (int64_t) n_head_kv) * std::max(head_dim, head_dim_v) > INT32_MAX / 2)
+        return IIAN_PA_ERR_ARG;
+    const int esize = row_type_bytes(r.type);
+    if (!esize) return IIAN_PA_ERR_UNSUPPORTED;
+    const int64_t qw = (int64_t) n_head * head_dim, kw = (int64_t) n_head_kv * head_dim;
+    if ((r.q && (r.q_stride < qw || r.q_out_stride < qw)) || r.k_stride < kw || (r.k_out && r.k_out_stride < kw) ||
+        (pools && r.v_stride < (int64_t) n_head_kv * head_dim_v))
+        return IIAN_PA_ERR_ARG;
+    // in place only row for row
+    if ((r.q && r.q_out == r.q && r.q_out_stride != r.q_stride) || (r.k_out == r.k && r.k_out_stride != r.k_stride))
+        return IIAN_PA_ERR_ARG;
+    if (((uintptr_t) r.q | (uintptr_t) r.k | (uintptr_t) r.q_out | (uintptr_t) r.k_out) & (esize - 1))
+        return IIAN_PA_ERR_ARG;
+    if (((uintptr_t) r.q_norm | (uintptr_t) r.k_norm | (uintptr_t) pos | (uintptr_t) axis) & 3 || (uintptr_t) freqs & 7)
+        return IIAN_PA_ERR_ARG;
+    if (pools) {
+        int64_t kb, vb;
+        int rc = row_bytes(type_k, kw, kb);
+        if (rc) return rc;
+        rc = row_bytes(type_v, (int64_t) n_head_kv * head_dim_v, vb);
+        if (rc) return rc;
+        if (!head_size_ok(type_k, head_dim) || !head_size_ok(type_v, head_dim_v)) return IIAN_PA_ERR_UNSUPPORTED;
+        auto align = [](int t) { return t == IIAN_PA_TYPE_F32 ? 3 : 1; };
+        if ((uintptr_t) r.v & (esize - 1) || (uintptr_t) k_pool & align(type_k) || (uintptr_t) v_pool & align(type_v) ||
+            (uintptr_t) slots & 7)
+            return IIAN_PA_ERR_ARG;
+    }
+    MropeParams p = {};
+    p.q = r.q;
+    p.k = r.k;
+    p.v = r.v;
+    p.q_out = r.q_out;
+    p.k_out = r.k_out;
+    p.q_stride = r.q_stride;
+    p.k_stride = r.k_stride;
+    p.v_stride = r.v_stride;
+    p.qo_stride = r.q_out_stride;
+    p.ko_stride = r.k_out_stride;
+    p.q_norm = r.q ? r.q_norm : nullptr;
+    p.k_norm = r.k_norm;
+    p.pos = pos;
+    p.slots = slots;
+    p.freqs = freqs;
+    p.axis = axis;
+    p.k_pool = k_pool;
+    p.v_pool = v_pool;
+    p.err = err_flag;
+    p.n_cells = n_cells;
+    p.eps = r.norm_eps;
+    p.mscale = mscale;
+    p.T = (int32_t) n_rows;
+    p.H = n_head;
+    p.Hkv = n_head_kv;
+    p.D = head_dim;
+    p.Dv = head_dim_v;
+    p.n_dims = n_dims;
+    p.mode = mode;
+    p.n_axes = n_axes;
+    p.type = r.type;
+    p.type_k = type_k;
+    p.type_v = type_v;
+    return launch_mrope_kv_write(p, (hipStream_t) stream) == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
+}
+
+int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const void *v, int type, int64_t q_stride,
+                             int64_t k_stride, int64_t v_stride, const int32_t *query_start_loc,
+                             const int32_t *row_end, int32_t n_tokens, int32_t n_seqs, int32_t max_query_len,
+                             int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v, float scale,
+                             float softcap, int32_t causal, int32_t n_swa, void *out, int64_t out_stride,
+                             int32_t *err_flag) {
+    if (n_tokens < 0 || n_seqs < 0 || max_query_len < 0) return IIAN_PA_ERR_ARG;
+    if (n_tokens == 0 || n_seqs == 0) return IIAN_PA_OK;
+    if (!q || !k || !v || !query_start_loc || !out) return IIAN_PA_ERR_NULL;
+    if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv || head_dim <= 0 || head_dim_v <= 0 ||
+        max_query_len == 0 || max_query_len > n_tokens || n_tokens > kMaxPromptTokens)
+        return IIAN_PA_ERR_ARG;
+    if (n_swa < 0 || softcap < 0.0f || !std::isfinite(scale) || !std::isfinite(softcap)) return IIAN_PA_ERR_ARG;
+    const int esize = row_type_bytes(type);
+    if (!esize || head_dim > kMaxHeadDim || head_dim_v > kMaxHeadDim) return IIAN_PA_ERR_UNSUPPORTED;
+    if ((int64_t) n_head * std::max(head_dim, head_dim_v) > INT32_MAX / 2 || (int64_t) n_tokens * n_head > INT32_MAX)
+        return IIAN_PA_ERR_ARG;
+    if (q_stride < (int64_t) n_head * head_dim || k_stride < (int64_t) n_head_kv * head_dim ||
+        v_stride < (int64_t) n_head_kv * head_dim_v || out_stride < (int64_t) n_head * head_dim_v)
+        return IIAN_PA_ERR_ARG;
+    if (((uintptr_t) q | (uintptr_t) k | (uintptr_t) v | (uintptr_t) out) & (esize - 1) ||
+        ((uintptr_t) query_start_loc | (uintptr_t) row_end) & 3)
+        return IIAN_PA_ERR_ARG;
+    PromptParams p = {};
+    p.q = q;
+    p.k = k;
+    p.v = v;
+    p.out = out;
+    p.q_stride = q_stride;
+    p.k_stride = k_stride;
+    p.v_stride = v_stride;
+    p.o_stride = out_stride;
+    p.qsl = query_start_loc;
+    p.row_end = row_end;
+    p.err = err_flag;
+    p.T = n_tokens;
+    p.S = n_seqs;
+    p.max_q = max_query_len;
+    p.H = n_head;
+    p.Hkv = n_head_kv;
+    p.gqa = n_head / n_head_kv;
+    p.D = head_dim;
+    p.Dv = head_dim_v;
+    p.scale = scale;
+    p.softcap = softcap;
+    p.causal = causal ? 1 : 0;
+    p.n_swa = n_swa;
+    return launch_prompt_rows(p, type, (hipStream_t) stream) == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
 }
 
 int iian_pa_dequant_q8_0(void *stream, const void *pool, int64_t n_cells, const int64_t *rows_idx, int64_t n_rows,

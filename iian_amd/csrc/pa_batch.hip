@@ -21,6 +21,8 @@
 #include "pa_common.h"
 #include "pa_launch.h"
 
+#include <algorithm>
+
 namespace iian_pa {
 
 __global__ __launch_bounds__(256) void pa_build_batch_kernel(BatchParams p) {
@@ -107,6 +109,160 @@ __global__ __launch_bounds__(256) void pa_swa_free_kernel(const int32_t *__restr
     if (lane == 0) n_free[s] = nf;
     if (block_tables)
         for (int b = lane; b < min(nf, max_blocks); b += 64) block_tables[(int64_t) s * max_blocks + b] = -1;
+}
+
+// Positions on three axes of a step's new tokens (iian_pa_mrope_positions).
+//
+// Workgroup (s, c) takes the c-th share of request s' new tokens.  It needs the
+// token and position prefix sums over the request's runs up to them: kRunsPer
+// runs per thread, loaded together and summed, a wave scan over the threads and
+// one over the waves, so a round covers 2048 runs and a request of 2000 takes
+// one.  The prefixes go to LDS, where each of the share's tokens finds its run
+// by a binary search.  Every share scans for itself: a request's runs are a few
+// KB and stay in L2, while a scan in a launch of its own would cost the launch.
+// Latency-bound: query_start_loc and span_off, then the runs, then the store.
+constexpr int kRunsPer = 8;
+constexpr int kRunsRound = 256 * kRunsPer;
+
+struct RunExtent {
+    int64_t tokens, advance;
+    bool bad;
+};
+
+// Tokens and position advance of a run, each below 2^31 (a larger one is held
+// at INT32_MAX: prefix sums of 2^31 runs stay within 64 bits).
+__device__ __forceinline__ RunExtent run_extent(const int4 &r) {
+    RunExtent e = {0, 0, false};
+    const bool grid = r.y != 0 || r.z != 0;
+    if (r.x < 0 || (grid && (r.y <= 0 || r.z <= 0))) {
+        e.bad = true;
+    } else if (!grid) {
+        e.tokens = e.advance = r.x;
+    } else if (r.x > 0) {
+        const int64_t plane = min((int64_t) r.y * r.z, (int64_t) INT32_MAX);
+        e.tokens = min(r.x * plane, (int64_t) INT32_MAX);
+        const int64_t time = (int64_t) (r.x - 1) * max(r.w, 1) + 1;
+        e.advance = min(max(time, (int64_t) max(r.y, r.z)), (int64_t) INT32_MAX);
+        e.bad = r.w < 1 || r.x * plane > INT32_MAX || time > INT32_MAX;
+    }
+    return e;
+}
+
+__global__ __launch_bounds__(256) void pa_mrope_positions_kernel(MropePosParams p) {
+    __shared__ int64_t wave_sum[2][4];
+    // tokens and position before each run of the round, and after the last
+    __shared__ int32_t tok[kRunsRound + 1], at[kRunsRound + 1];
+    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int q0 = min(max(p.qsl[s], 0), p.T), q1 = min(max(p.qsl[s + 1], q0), p.T);
+    const int nn = q1 - q0;
+    // shares of whole waves
+    const int64_t per = ((int64_t) nn + gridDim.y - 1) / gridDim.y + 63 & ~(int64_t) 63;
+    const int i0 = (int) min(blockIdx.y * per, (int64_t) nn), i1 = (int) min(i0 + per, (int64_t) nn);
+    const int f0 = p.span_off[s], f1 = p.span_off[s + 1];
+    const int nc = p.num_computed[s];
+    const int b0 = min(max(f0, 0), p.n_spans), b1 = min(max(f1, b0), p.n_spans);
+    bool bad = nc < 0 || f0 != b0 || f1 != b1;
+    const bool first = blockIdx.y == 0;   // flags each request once, whether it has new tokens or not
+    if (i0 >= i1 && !first) return;
+    const int64_t r0 = (int64_t) max(nc, 0) + i0, r1 = (int64_t) max(nc, 0) + i1;   // the share's tokens of the request
+    int64_t tok0 = 0, at0 = 0;   // before the round
+    int64_t done = r0;           // tokens written so far
+    auto put = [&](int64_t r, int64_t pt, int64_t ph, int64_t pw, int64_t end) {
+        const int t = q0 + (int) (r - max(nc, 0));
+        bad |= pt > INT32_MAX || ph > INT32_MAX || pw > INT32_MAX || end > INT32_MAX;
+        p.pos[t] = (int32_t) min(pt, (int64_t) INT32_MAX);
+        p.pos[(int64_t) p.T + t] = (int32_t) min(ph, (int64_t) INT32_MAX);
+        p.pos[2 * (int64_t) p.T + t] = (int32_t) min(pw, (int64_t) INT32_MAX);
+        if (p.row_end) p.row_end[t] = (int32_t) min(end, (int64_t) INT32_MAX);
+    };
+    for (int b = b0; b < b1 && done < r1; b += kRunsRound) {
+        const int n = min(kRunsRound, b1 - b);
+        int4 run[kRunsPer];
+        int64_t ts = 0, as = 0;
+#pragma unroll
+        for (int k = 0; k < kRunsPer; k++) {
+            const int j = tid * kRunsPer + k;
+            run[k] = j < n ? p.spans[b + j] : make_int4(0, 0, 0, 1);
+        }
+#pragma unroll
+        for (int k = 0; k < kRunsPer; k++) {
+            const RunExtent e = run_extent(run[k]);
+            bad |= e.bad;
+            ts += e.tokens;
+            as += e.advance;
+        }
+        int64_t tp = ts, ap = as;   // inclusive scans over the wave's lanes
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t x = __shfl_up(tp, o), y = __shfl_up(ap, o);
+            if (lane >= o) {
+                tp += x;
+                ap += y;
+            }
+        }
+        if (lane == 63) {
+            wave_sum[0][wave] = tp;
+            wave_sum[1][wave] = ap;
+        }
+        __syncthreads();
+        int64_t tw = tok0, aw = at0;
+        for (int w = 0; w < 4; w++) {
+            if (w < wave) {
+                tw += wave_sum[0][w];
+                aw += wave_sum[1][w];
+            }
+            tok0 += wave_sum[0][w];
+            at0 += wave_sum[1][w];
+        }
+        tw += tp - ts;
+        aw += ap - as;
+#pragma unroll
+        for (int k = 0; k < kRunsPer; k++) {
+            tok[tid * kRunsPer + k] = (int32_t) min(tw, (int64_t) INT32_MAX);
+            at[tid * kRunsPer + k] = (int32_t) min(aw, (int64_t) INT32_MAX);
+            const RunExtent e = run_extent(run[k]);
+            tw += e.tokens;
+            aw += e.advance;
+        }
+        if (tid == 255) {
+            tok[kRunsRound] = (int32_t) min(tw, (int64_t) INT32_MAX);
+            at[kRunsRound] = (int32_t) min(aw, (int64_t) INT32_MAX);
+        }
+        __syncthreads();
+        const int64_t stop = min(r1, tok0);   // the round's runs hold tokens up to tok0
+        for (int64_t r = done + tid; r < stop; r += 256) {
+            // the last run that starts at or before token r: it holds r, since the
+            // runs of no tokens behind it start where the next one does
+            int lo = 0, hi = kRunsRound;
+            while (hi - lo > 1) {
+                const int m = (lo + hi) >> 1;
+                if (tok[m] <= r) lo = m;
+                else hi = m;
+            }
+            const int4 g = p.spans[b + min(lo, n - 1)];
+            const uint32_t i = (uint32_t) (r - tok[lo]);
+            const int64_t base = at[lo];
+            if (g.y > 0 && g.z > 0) {
+                const uint32_t w = (uint32_t) g.z, h = (uint32_t) g.y, row = i / w, it = row / h;
+                put(r, base + (int64_t) it * max(g.w, 1), base + (row - it * h), base + (i - row * w),
+                    p.grid_full ? (int64_t) tok[lo + 1] : r + 1);
+            } else {
+                put(r, base + i, base + i, base + i, r + 1);
+            }
+        }
+        done = max(done, stop);
+        __syncthreads();   // the prefixes are rewritten by the next round
+    }
+    for (int64_t r = done + tid; r < r1; r += 256) put(r, at0 + (r - tok0), at0 + (r - tok0), at0 + (r - tok0), r + 1);
+    if (bad && p.err) atomicOr(p.err, 8);
+}
+
+hipError_t launch_mrope_positions(const MropePosParams &p, hipStream_t stream) {
+    // Shares per request: one per 512 tokens of the step, up to 64 (a single
+    // request may hold them all); a share of no tokens ends at once.
+    const int shares = std::min(64, std::max(1, (p.T + 511) / 512));
+    hipLaunchKernelGGL(pa_mrope_positions_kernel, dim3(p.S, shares), dim3(256), 0, stream, p);
+    return hipGetLastError();
 }
 
 hipError_t launch_swa_free(const int32_t *qsl, const int32_t *pos, int32_t S, int32_t T, int32_t n_swa,

@@ -604,3 +604,5 @@ hipError_t launch_general(const GenParams &p, int type_k, int type_v, hipStream_
 }
 
 }  // namespace iian_pa
+
+#include "pa_prompt_rows.h"

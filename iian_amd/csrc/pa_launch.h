@@ -111,6 +111,19 @@ hipError_t launch_swa_free(const int32_t *qsl, const int32_t *pos, int32_t S, in
                            int32_t block_size, int32_t *n_free, int32_t *block_tables, int32_t max_blocks,
                            hipStream_t stream);
 
+// Inputs and outputs of the multi-axis positions kernel (pa_batch.hip).
+struct MropePosParams {
+    const int4 *spans;            // runs (t, h, w, step)
+    const int32_t *span_off;      // [S+1]
+    const int32_t *num_computed;  // [S]
+    const int32_t *qsl;           // [S+1]
+    int32_t *pos;                 // [3][T]
+    int32_t *row_end;             // nullable [T]
+    int32_t *err;                 // nullable
+    int32_t n_spans, S, T, grid_full;
+};
+hipError_t launch_mrope_positions(const MropePosParams &p, hipStream_t stream);
+
 // Inputs of the fused RoPE + KV write (pa_rope.hip).
 struct RopeParams {
     const float *k_rows;          // [T][Hkv*D] before RoPE
@@ -127,6 +140,40 @@ struct RopeParams {
     float theta_scale, freq_scale, ext_factor, mscale, corr0, corr1;
 };
 hipError_t launch_rope_kv_write(const RopeParams &p, int type_k, int type_v, hipStream_t stream);
+
+// Inputs of the multi-axis rotary KV write (pa_mrope.h); strides in elements of `type`.
+struct MropeParams {
+    const void *q, *k, *v;        // q nullable; v read when the pools are given
+    void *q_out, *k_out;          // k_out nullable
+    int64_t q_stride, k_stride, v_stride, qo_stride, ko_stride;
+    const float *q_norm, *k_norm; // nullable [D]
+    const int32_t *pos;           // [n_axes][T]
+    const int64_t *slots;         // [T]
+    const double *freqs;          // [n_dims/2], radians per position
+    const int32_t *axis;          // [n_dims/2]
+    void *k_pool, *v_pool;        // both NULL: no KV write
+    int32_t *err;
+    int64_t n_cells;
+    float eps, mscale;
+    int32_t T, H, Hkv, D, Dv, n_dims, mode, n_axes;
+    int32_t type, type_k, type_v;
+};
+hipError_t launch_mrope_kv_write(const MropeParams &p, hipStream_t stream);
+
+// Inputs of whole-prompt attention (pa_prompt.hip, pa_prompt_rows.h); strides in elements.
+struct PromptParams {
+    const void *q, *k, *v;
+    void *out;
+    int64_t q_stride, k_stride, v_stride, o_stride;
+    const int32_t *qsl;           // [S+1]
+    const int32_t *row_end;       // nullable [T]
+    int32_t *err;
+    int32_t T, S, max_q, H, Hkv, gqa, D, Dv;
+    float scale, softcap;
+    int32_t causal, n_swa;
+};
+// One wave per (token, head), any head size and alignment (pa_general.hip).
+hipError_t launch_prompt_rows(const PromptParams &p, int type, hipStream_t stream);
 
 // General fp32 path (pa_general.hip): any K/V types of F32, F16, Q8_0; head
 // sizes 4..512 in steps of 4; any block size.

@@ -434,3 +434,5 @@ hipError_t launch_rope_kv_write(const RopeParams &p, int type_k, int type_v, hip
 }
 
 }  // namespace iian_pa
+
+#include "pa_mrope.h"

@@ -662,3 +662,245 @@ def dequant_q8_0(pool: KVPool, rows_idx: torch.Tensor) -> torch.Tensor:
                                           rows_idx.shape[0], pool.n_embd, out.data_ptr())
     _lib.check("iian_pa_dequant_q8_0", st)
     return out
+
+
+# ---- Prompts with images or video: positions of several axes ----
+
+MROPE_SECTIONS = _lib.MROPE_SECTIONS
+MROPE_INTERLEAVED = _lib.MROPE_INTERLEAVED
+MROPE_RESTART = _lib.MROPE_RESTART
+_ROW_TYPES = {torch.float32: _lib.TYPE_F32, torch.float16: _lib.TYPE_F16, torch.bfloat16: _lib.TYPE_BF16}
+
+
+def _bound(name: str, args: tuple, keep: object = None) -> Callable[[], None]:
+    """A function that issues entry point `name` again with these arguments."""
+    fn = getattr(_lib.load(), name)
+
+    def call() -> None:
+        st = fn(*args)
+        if st:
+            _lib.check(name, st)
+    call.keep = keep   # what the arguments point at
+    return call
+
+
+def _int_array(name: str, t: torch.Tensor, shape: tuple, device: torch.device, dtype=torch.int32) -> None:
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on {device}")
+
+
+def _call_ok(err_flag: Optional[torch.Tensor], device: torch.device) -> None:
+    # (the stream is the current device's: a call for another one would not run there)
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {device}, but the current device is {torch.cuda.current_device()}")
+    if err_flag is not None and (err_flag.dtype != torch.int32 or err_flag.numel() < 1 or err_flag.device != device):
+        raise ValueError("err_flag must be an int32 tensor on the rows' device")
+
+
+def _positions_args(spans, span_off, num_computed, query_start_loc, pos, row_end, grid_full, err_flag):
+    dev = spans.device
+    if not spans.is_cuda or spans.dim() != 2 or spans.shape[1] != 4:
+        raise ValueError("spans must be a GPU tensor [n_spans, 4] of runs (t, h, w, step)")
+    S = int(num_computed.shape[0]) if num_computed.dim() == 1 else -1
+    _int_array("spans", spans, (spans.shape[0], 4), dev)
+    _int_array("num_computed", num_computed, (S,), dev)
+    _int_array("span_off", span_off, (S + 1,), dev)
+    _int_array("query_start_loc", query_start_loc, (S + 1,), dev)
+    if pos.dim() != 2:
+        raise ValueError("pos must be [3, n_tokens]")
+    T = int(pos.shape[1])
+    _int_array("pos", pos, (3, T), dev)
+    if row_end is not None:
+        _int_array("row_end", row_end, (T,), dev)
+    _call_ok(err_flag, dev)
+    return (_stream(), spans.data_ptr(), span_off.data_ptr(), int(spans.shape[0]), num_computed.data_ptr(),
+            query_start_loc.data_ptr(), S, T, int(bool(grid_full)), pos.data_ptr(), _ptr(row_end), _ptr(err_flag))
+
+
+def mrope_positions(spans: torch.Tensor, span_off: torch.Tensor, num_computed: torch.Tensor,
+                    query_start_loc: torch.Tensor, pos: torch.Tensor, row_end: Optional[torch.Tensor] = None,
+                    grid_full: bool = False, err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Positions on three axes of a step's new tokens into pos (int32
+    [3, n_tokens]), from each request's runs of text and grids, and what each
+    token may attend into row_end (iian_pa_mrope_positions): request s is
+    spans[span_off[s]:span_off[s + 1]], int32 (t, h, w, step) each, and brings
+    its tokens num_computed[s], ... at query_start_loc[s]."""
+    args = _positions_args(spans, span_off, num_computed, query_start_loc, pos, row_end, grid_full, err_flag)
+    _lib.check("iian_pa_mrope_positions", _lib.load().iian_pa_mrope_positions(*args))
+    return pos
+
+
+def bind_mrope_positions(spans: torch.Tensor, span_off: torch.Tensor, num_computed: torch.Tensor,
+                         query_start_loc: torch.Tensor, pos: torch.Tensor, row_end: Optional[torch.Tensor] = None,
+                         grid_full: bool = False, err_flag: Optional[torch.Tensor] = None) -> Callable[[], None]:
+    """mrope_positions checked once and bound to these buffers and the current
+    stream, as bind_paged_attn."""
+    return _bound("iian_pa_mrope_positions", _positions_args(spans, span_off, num_computed, query_start_loc, pos,
+                                                             row_end, grid_full, err_flag))
+
+
+def mrope_frequencies(rope: RopeParams, sections: Sequence[int], layout: int = MROPE_SECTIONS, device="cuda"):
+    """(freqs float64 [n_dims/2], axis int32 [n_dims/2], mscale) of a multi-axis
+    rotary embedding (iian_pa_mrope_frequencies), once per model.  rope.mode is
+    not used; rope.freq_factors may be on any device."""
+    if not 1 <= len(sections) <= 4:
+        raise ValueError("1 to 4 sections")
+    half = max(0, rope.n_dims // 2)
+    ff = None
+    if rope.freq_factors is not None:
+        ff = rope.freq_factors.detach().to("cpu", torch.float32).contiguous()
+        if ff.numel() < half:
+            raise ValueError("freq_factors must hold n_dims/2 values")
+    prm = _lib.RopeParams(rope.n_dims, rope.mode, rope.n_ctx_orig, rope.freq_base, rope.freq_scale, rope.ext_factor,
+                          rope.attn_factor, rope.beta_fast, rope.beta_slow, _ptr(ff))
+    ax = _lib.MRopeAxes(len(sections), layout, (C.c_int32 * 4)(*sections))
+    freqs, axis, ms = np.zeros(max(half, 1)), np.zeros(max(half, 1), np.int32), C.c_float(0)
+    _lib.check("iian_pa_mrope_frequencies", _lib.load().iian_pa_mrope_frequencies(
+        C.byref(prm), C.byref(ax), freqs.ctypes.data, axis.ctypes.data, C.byref(ms)))
+    return torch.as_tensor(freqs).to(device), torch.as_tensor(axis).to(device), float(ms.value)
+
+
+def _head_rows(name: str, t: torch.Tensor, T: int, like: torch.Tensor) -> int:
+    """Token stride of rows [T, heads, size] whose tokens' heads are contiguous."""
+    if t.dim() != 3 or t.shape[0] != T or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be [{T}, heads, head size] of {like.dtype} on {like.device}")
+    if (t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError(f"{name}: the heads of a token must be contiguous")
+    return max(int(t.stride(0)), int(t.shape[1] * t.shape[2])) if T <= 1 else int(t.stride(0))
+
+
+def _mrope_args(k_pool, v_pool, k_rows, v_rows, slots, pos, freqs, axis, q, q_out, k_out, neox, q_norm, k_norm,
+                norm_eps, mscale, err_flag):
+    if k_rows.dtype not in _ROW_TYPES or k_rows.dim() != 3 or not k_rows.is_cuda:
+        raise ValueError("k_rows must be an f32, f16 or bf16 GPU tensor [n_tokens, n_head_kv, head_dim]")
+    T, Hkv, D = k_rows.shape
+    dev = k_rows.device
+    r = _lib.MRopeRows()
+    r.type = _ROW_TYPES[k_rows.dtype]
+    r.norm_eps = float(norm_eps)
+    r.k, r.k_stride = k_rows.data_ptr(), _head_rows("k_rows", k_rows, T, k_rows)
+    H, Dv = 0, D
+    if q is not None:
+        r.q, r.q_stride = q.data_ptr(), _head_rows("q", q, T, k_rows)
+        H = int(q.shape[1])
+        if q_out is None or tuple(q_out.shape) != tuple(q.shape) or q.shape[2] != D:
+            raise ValueError("q and q_out must be [n_tokens, n_head, head_dim]")
+        r.q_out, r.q_out_stride = q_out.data_ptr(), _head_rows("q_out", q_out, T, k_rows)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if k_out is not None:
+        if tuple(k_out.shape) != tuple(k_rows.shape):
+            raise ValueError("k_out must be shaped like k_rows")
+        r.k_out, r.k_out_stride = k_out.data_ptr(), _head_rows("k_out", k_out, T, k_rows)
+    if (k_pool is None) != (v_pool is None) or (k_pool is None) != (slots is None):
+        raise ValueError("k_pool, v_pool and slots go together")
+    if k_pool is not None:
+        if v_rows is None:
+            raise ValueError("v_rows to write")
+        r.v, r.v_stride = v_rows.data_ptr(), _head_rows("v_rows", v_rows, T, k_rows)
+        Dv = int(v_rows.shape[2])
+        if v_rows.shape[1] != Hkv or k_pool.n_embd != Hkv * D or v_pool.n_embd != Hkv * Dv:
+            raise ValueError("pool rows must hold the rows' kv heads")
+        if k_pool.n_cells != v_pool.n_cells or k_pool.data.device != dev or v_pool.data.device != dev:
+            raise ValueError("pools must hold the same number of cells, on the rows' device")
+        _int_array("slots", slots, (T,), dev, torch.int64)
+    elif k_out is None:
+        raise ValueError("neither pools nor k_out to write K to")
+    half = int(freqs.shape[0]) if freqs.dim() == 1 else -1
+    _int_array("freqs", freqs, (half,), dev, torch.float64)
+    _int_array("axis", axis, (half,), dev)
+    if pos.dim() != 2:
+        raise ValueError("pos must be [n_axes, n_tokens]")
+    _int_array("pos", pos, (pos.shape[0], T), dev)
+    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if w is not None and (w.dtype != torch.float32 or tuple(w.shape) != (D,) or not w.is_contiguous() or w.device != dev):
+            raise ValueError(f"{name} must be contiguous f32 [{D}] on the rows' device")
+    r.q_norm, r.k_norm = _ptr(q_norm), _ptr(k_norm)
+    _call_ok(err_flag, dev)
+    return (_stream(), C.byref(r), pos.data_ptr(), _ptr(slots), T, H, Hkv, D, Dv, freqs.data_ptr(), axis.data_ptr(),
+            int(pos.shape[0]), 2 * half, 2 if neox else 0, float(mscale),
+            k_pool.data.data_ptr() if k_pool is not None else None,
+            v_pool.data.data_ptr() if v_pool is not None else None, k_pool.n_cells if k_pool is not None else 0,
+            k_pool.type if k_pool is not None else GGML_TYPE_F16, v_pool.type if v_pool is not None else GGML_TYPE_F16,
+            _ptr(err_flag)), r
+
+
+def mrope_set_rows_kv(k_pool: Optional[KVPool], v_pool: Optional[KVPool], k_rows: torch.Tensor,
+                      v_rows: Optional[torch.Tensor], slots: Optional[torch.Tensor], pos: torch.Tensor,
+                      freqs: torch.Tensor, axis: torch.Tensor, q: Optional[torch.Tensor] = None,
+                      q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None, neox: bool = True,
+                      q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None,
+                      norm_eps: float = 1e-6, mscale: float = 1.0,
+                      err_flag: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Multi-axis RoPE of K (and q) behind the heads' RMS norm (where weights are
+    given), and the K/V write, in one launch (iian_pa_mrope_kv_write).  Rows are
+    [n_tokens, heads, head size] of f32, f16 or bf16, tokens any stride apart;
+    pos int32 [n_axes, n_tokens]; freqs and axis as mrope_frequencies gives
+    them.  The rotated rows go to q_out (a new tensor when None), k_out and the
+    pools; without pools (a vision tower) k_out takes K alone.  Returns q_out."""
+    if q is not None and q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    args, _rows = _mrope_args(k_pool, v_pool, k_rows, v_rows, slots, pos, freqs, axis, q, q_out, k_out, neox, q_norm,
+                              k_norm, norm_eps, mscale, err_flag)
+    _lib.check("iian_pa_mrope_kv_write", _lib.load().iian_pa_mrope_kv_write(*args))
+    return q_out
+
+
+def bind_mrope_set_rows_kv(k_pool: Optional[KVPool], v_pool: Optional[KVPool], k_rows: torch.Tensor,
+                           v_rows: Optional[torch.Tensor], slots: Optional[torch.Tensor], pos: torch.Tensor,
+                           freqs: torch.Tensor, axis: torch.Tensor, q: Optional[torch.Tensor] = None,
+                           q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                           neox: bool = True, q_norm: Optional[torch.Tensor] = None,
+                           k_norm: Optional[torch.Tensor] = None, norm_eps: float = 1e-6, mscale: float = 1.0,
+                           err_flag: Optional[torch.Tensor] = None) -> Callable[[], None]:
+    """mrope_set_rows_kv checked once and bound to these buffers (q_out given
+    when q is) and the current stream, as bind_paged_attn."""
+    args, rows = _mrope_args(k_pool, v_pool, k_rows, v_rows, slots, pos, freqs, axis, q, q_out, k_out, neox, q_norm,
+                             k_norm, norm_eps, mscale, err_flag)
+    return _bound("iian_pa_mrope_kv_write", args, rows)
+
+
+def _prompt_args(q, k, v, query_start_loc, max_query_len, params, out, row_end, err_flag):
+    if q.dtype not in _ROW_TYPES or q.dim() != 3 or not q.is_cuda:
+        raise ValueError("q must be an f32, f16 or bf16 GPU tensor [n_tokens, n_head, head_dim]")
+    T, H, D = q.shape
+    strides = [_head_rows(n, t, T, q) for n, t in (("q", q), ("k", k), ("v", v), ("out", out))]
+    Hkv, Dv = int(k.shape[1]), int(v.shape[2])
+    if k.shape[2] != D or v.shape[1] != Hkv or tuple(out.shape) != (T, H, Dv):
+        raise ValueError("k must be [T, n_head_kv, head_dim], v [T, n_head_kv, head_dim_v], out [T, n_head, head_dim_v]")
+    if query_start_loc.dim() != 1 or query_start_loc.shape[0] < 1:
+        raise ValueError("query_start_loc must have n_seqs + 1 entries")
+    _int_array("query_start_loc", query_start_loc, (query_start_loc.shape[0],), q.device)
+    if row_end is not None:
+        _int_array("row_end", row_end, (T,), q.device)
+    _call_ok(err_flag, q.device)
+    return (_stream(), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ROW_TYPES[q.dtype], *strides[:3],
+            query_start_loc.data_ptr(), _ptr(row_end), T, int(query_start_loc.shape[0]) - 1, int(max_query_len), H, Hkv,
+            D, Dv, float(params.scale), float(params.softcap), int(bool(params.causal)), int(params.n_swa),
+            out.data_ptr(), strides[3], _ptr(err_flag))
+
+
+def prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_start_loc: torch.Tensor, max_query_len: int,
+                params: PagedAttnParams, out: Optional[torch.Tensor] = None, row_end: Optional[torch.Tensor] = None,
+                err_flag: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention over whole prompts with nothing before them, from their rows
+    (iian_pa_prompt_attention): q [T, H, D], k [T, Hkv, D], v [T, Hkv, Dv] of f32,
+    f16 or bf16, tokens any stride apart, prompts packed behind each other at
+    query_start_loc (int32 [n_seqs + 1]).  row_end (int32 [T], mrope_positions'
+    say) replaces the causal bound where given.  Returns out [T, H, Dv] of q's
+    type; rows outside every prompt are left as they were."""
+    if out is None:
+        out = torch.empty((q.shape[0], q.shape[1], v.shape[2]), dtype=q.dtype, device=q.device)
+    args = _prompt_args(q, k, v, query_start_loc, max_query_len, params, out, row_end, err_flag)
+    _lib.check("iian_pa_prompt_attention", _lib.load().iian_pa_prompt_attention(*args))
+    return out
+
+
+def bind_prompt_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_start_loc: torch.Tensor,
+                     max_query_len: int, params: PagedAttnParams, out: torch.Tensor,
+                     row_end: Optional[torch.Tensor] = None,
+                     err_flag: Optional[torch.Tensor] = None) -> Callable[[], None]:
+    """prompt_attn checked once and bound to these buffers and the current
+    stream, as bind_paged_attn."""
+    return _bound("iian_pa_prompt_attention", _prompt_args(q, k, v, query_start_loc, max_query_len, params, out,
+                                                           row_end, err_flag))

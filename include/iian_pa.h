@@ -51,6 +51,10 @@ enum {
 
 enum { IIAN_PA_TYPE_F32 = 0, IIAN_PA_TYPE_F16 = 1, IIAN_PA_TYPE_Q8_0 = 8 };
 
+/* BF16 rows (ggml's type code), taken by iian_pa_mrope_kv_write and
+ * iian_pa_prompt_attention only; no pool type. */
+enum { IIAN_PA_TYPE_BF16 = 30 };
+
 /* Human-readable text of a status code (static storage). */
 const char *iian_pa_status_string(int status);
 
@@ -291,6 +295,132 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
                           int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v,
                           const iian_pa_rope_params *rope, void *k_pool, void *v_pool, int64_t n_cells,
                           int type_k, int type_v, int32_t *err_flag);
+
+/* ---- Prompts with images or video: positions of several axes ----
+ *
+ * A multimodal prompt gives each token a position on three axes (time, height,
+ * width), and each pair of a head's values turns by its own axis' position.
+ * iian_pa_mrope_positions derives the positions of a step's tokens from each
+ * request's content, iian_pa_mrope_kv_write rotates and writes the step's
+ * rows, and attention follows: iian_pa_attention over the pool, whose
+ * masks go by token index (iian_pa_build_batch's pos) as ever, or, for prompts
+ * with nothing before them, iian_pa_prompt_attention over the rows themselves.
+ * The reference has no counterpart. */
+
+/* Positions of a step's new tokens on three axes, from what each request
+ * consists of.  Request s is the runs spans[span_off[s] .. span_off[s+1]) in
+ * order, each int32 (t, h, w, step):
+ *   h == w == 0   t tokens of text; token i has position p + i on every axis, and p grows by t
+ *   h, w > 0      a grid of t*h*w tokens, width fastest: token (it, ih, iw) has positions
+ *                 (p + it*step, p + ih, p + iw), and p grows by max((t-1)*step + 1, h, w)
+ * with p = 0 at the request's start; a run of no tokens leaves p as it is, and
+ * tokens past the last run are text (a decode step needs no new runs).  Tokens
+ * [query_start_loc[s], query_start_loc[s+1]) of the step are the request's
+ * tokens num_computed[s], num_computed[s] + 1, ...
+ *   pos      int32 [3][n_tokens]: time, height, width
+ *   row_end  int32 [n_tokens], nullable: the number of the request's leading
+ *            tokens that the token may attend: its own index + 1, or, with
+ *            grid_full != 0, all through its grid's last one
+ * Rows past query_start_loc[S] are left as they were.  All arrays are device
+ * memory.  *err_flag (when non-NULL) bit 3: a negative count or size, a grid
+ * with h or w zero or a step below 1 (its tokens then count as none, its step
+ * as 1), offsets out of order or outside [0, n_spans], or a position or end
+ * past INT32_MAX, which is held there. */
+int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
+                            const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
+                            int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag);
+
+/* Which axis each pair of a head turns by. */
+enum {
+    IIAN_PA_MROPE_SECTIONS = 0,     /* the first sections[0] pairs by axis 0, the next sections[1] by axis 1, ... */
+    IIAN_PA_MROPE_INTERLEAVED = 1,  /* axes take turns: pair j by axis j % n_axes while j < n_axes*sections[j % n_axes],
+                                       else by axis 0 */
+    IIAN_PA_MROPE_RESTART = 2       /* as SECTIONS, each section with a whole set of frequencies of its own:
+                                       freq_base^(-i/sections[a]) for its i-th pair (vision towers) */
+};
+
+typedef struct {
+    int32_t n_axes;        /* 1 .. 4 */
+    int32_t layout;
+    int32_t sections[4];   /* pairs per axis; their sum is n_dims/2 */
+} iian_pa_mrope_axes;
+
+/* Frequencies of a model's multi-axis rotary embedding, once, on the host: for
+ * pair j < n_dims/2, freqs[j] in radians per position, computed in 64 bits from
+ * rope's n_dims, freq_base, freq_scale, YaRN parameters (as
+ * iian_pa_rope_kv_write uses them) and freq_factors (here host memory), and
+ * axis[j]; *mscale (nullable) receives the magnitude scale.  The caller uploads
+ * both arrays; any frequencies and axes of its own do as well.  YaRN
+ * (ext_factor != 0) with IIAN_PA_MROPE_RESTART is IIAN_PA_ERR_UNSUPPORTED. */
+int iian_pa_mrope_frequencies(const iian_pa_rope_params *rope, const iian_pa_mrope_axes *axes, double *freqs,
+                              int32_t *axis, float *mscale);
+
+/* Rows of one layer, as its projections wrote them: q [T][n_head][head_dim],
+ * k [T][n_head_kv][head_dim], v [T][n_head_kv][head_dim_v], each token's heads
+ * contiguous, tokens *_stride elements apart (a fused projection's rows, say). */
+typedef struct {
+    const void *q;             /* nullable, with q_out */
+    const void *k;
+    const void *v;             /* read when the pools are given */
+    void *q_out;               /* rotated q; may be q itself with the same stride */
+    void *k_out;               /* nullable: rotated K rows; may be k itself with the same stride */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+    const float *q_norm;       /* nullable: weights [head_dim] of an RMS norm of each q head before the rotation */
+    const float *k_norm;       /* nullable: of each K head */
+    float norm_eps;
+    int32_t type;              /* of all five: IIAN_PA_TYPE_F32, _F16 or _BF16 */
+} iian_pa_mrope_rows;
+
+/* Multi-axis RoPE of K (and q), the heads' RMS norm before it where weights
+ * are given, and the slot-mapped K/V write, in one launch: for every token t
+ *   x = q or k head;  x <- x / sqrt(mean(x^2) + norm_eps) * weight   (with weights)
+ *   pair j turns by the angle pos[axis[j]][t] * freqs[j], scaled by mscale:
+ *     (x0, x1) <- mscale * (x0 cos - x1 sin, x0 sin + x1 cos)
+ *   q_out[t], k_out[t] <- the rotated rows, rounded to `type`
+ *   k_pool row slots[t] <- convert(rotated k), v_pool row slots[t] <- convert(v[t])
+ * Arithmetic is fp32 without a rounding in between (the pool's values come from
+ * the fp32 result, not from k_out); the angle is reduced exactly, so far
+ * positions are as precise as near ones.  mode is rope's: 0 pairs (2j, 2j+1),
+ * 2 pairs (j, j + n_dims/2); values past n_dims are copied (normed, not scaled).
+ *   pos    int32 [n_axes][n_rows]; any value, negative ones included
+ *   freqs  double [n_dims/2], axis int32 [n_dims/2] (device; an axis outside
+ *          [0, n_axes) is taken as the nearest one inside)
+ * The pools, their types, slots and *err_flag bit 0 are iian_pa_kv_write's;
+ * k_pool, v_pool and slots may all be NULL when k_out is given (a vision
+ * tower keeps no cache; v is not read then).  Buffers must be aligned to their
+ * element, pools to 2 bytes (Q8_0) or their element.  Head sizes 1 to 1024
+ * (multiples of 32 for a Q8_0 pool), n_dims even and at most head_dim. */
+int iian_pa_mrope_kv_write(void *stream, const iian_pa_mrope_rows *rows, const int32_t *pos, const int64_t *slots,
+                           int64_t n_rows, int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v,
+                           const double *freqs, const int32_t *axis, int32_t n_axes, int32_t n_dims, int32_t mode,
+                           float mscale, void *k_pool, void *v_pool, int64_t n_cells, int type_k, int type_v,
+                           int32_t *err_flag);
+
+/* Attention over whole prompts with nothing before them, from the rows
+ * themselves: n_seqs prompts packed behind each other, tokens
+ * [query_start_loc[s], query_start_loc[s+1]) of prompt s attending its own
+ * tokens.  For token i (counted from its prompt's start) and head h,
+ *   out = sum_j softmax_j(s_ij) v_j,  s_ij = scale * <q_i, k_j> (softcap as iian_pa_attention's),
+ * over the tokens j of its prompt with j < end_i and, when n_swa > 0,
+ * i - j < n_swa; end_i is row_end[i] where row_end is given (int32 [T], clamped
+ * to [0, prompt length]), else i + 1 (causal) or the prompt's length.  A
+ * token that sees none gets a zero row.  Rows outside every prompt are neither
+ * read nor written.  A value of k or v that a token does not see never reaches
+ * its output, infinities and NaN included.
+ *   q [T][n_head][head_dim], k [T][n_head_kv][head_dim], v [T][n_head_kv][head_dim_v],
+ *   out [T][n_head][head_dim_v], all of `type` (F32, F16 or BF16), tokens of
+ *   q, k, v and out *_stride elements apart; aligned to their element
+ *   max_query_len  host int: the longest prompt's tokens (or more); rows of a
+ *                  longer one past it may be left unwritten and set bit 2 of *err_flag
+ * Scores, sums and softmax statistics are fp32; F16 and BF16 rows enter the
+ * matrix products as they are and probabilities rounded to their type, F32
+ * rows as pairs of f16 terms (22 bits).  Head sizes 1 to 1024.  No workspace. */
+int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const void *v, int type, int64_t q_stride,
+                             int64_t k_stride, int64_t v_stride, const int32_t *query_start_loc,
+                             const int32_t *row_end, int32_t n_tokens, int32_t n_seqs, int32_t max_query_len,
+                             int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v, float scale,
+                             float softcap, int32_t causal, int32_t n_swa, void *out, int64_t out_stride,
+                             int32_t *err_flag);
 
 /* ---- Engine runtime: the integration point for an engine with its KV cache on the GPU ----
  *
