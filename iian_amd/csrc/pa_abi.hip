@@ -1104,7 +1104,7 @@ int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const v
     p.softcap = softcap;
     p.causal = causal ? 1 : 0;
     p.n_swa = n_swa;
-    return launch_prompt_rows(p, type, (hipStream_t) stream) == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
+    return launch_prompt(p, type, (hipStream_t) stream) == hipSuccess ? IIAN_PA_OK : IIAN_PA_ERR_HIP;
 }
 
 int iian_pa_dequant_q8_0(void *stream, const void *pool, int64_t n_cells, const int64_t *rows_idx, int64_t n_rows,

@@ -172,6 +172,11 @@ struct PromptParams {
     float scale, softcap;
     int32_t causal, n_swa;
 };
+// Matrix-core kernels at head sizes up to 256, the row form above (pa_prompt.hip).
+hipError_t launch_prompt(const PromptParams &p, int type, hipStream_t stream);
+hipError_t launch_prompt_f16(const PromptParams &p, hipStream_t stream);
+hipError_t launch_prompt_bf16(const PromptParams &p, hipStream_t stream);
+hipError_t launch_prompt_f32(const PromptParams &p, hipStream_t stream);
 // One wave per (token, head), any head size and alignment (pa_general.hip).
 hipError_t launch_prompt_rows(const PromptParams &p, int type, hipStream_t stream);
 

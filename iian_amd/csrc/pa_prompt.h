@@ -1,0 +1,606 @@
+// pa_prompt.h - whole-prompt attention on the matrix cores (iian_pa_prompt_attention):
+// packed prompts, grouped heads, head sizes up to 256; F16, BF16 and F32 rows
+// (pa_prompt.hip, pa_prompt_bf16.hip, pa_prompt_f32.hip hold one type each).
+//
+// A workgroup of 4 waves owns 128 rows r = i*gqa + g (token i, head g of the
+// group) of one (prompt, kv head), 32 per wave, and walks the tokens that any of
+// them sees in tiles of KT, staged in LDS (two buffers, one barrier per tile: the
+// next tile's rows are requested before the tile is computed and written behind
+// it).  One pass with a running maximum and sum per row:
+//
+//   S^T = K Q^T     v_mfma_f32_32x32x16: K rows are the A operand as they lie in
+//                   LDS, Q^T stays in registers.  Lane l then holds, of row l%32,
+//                   the scores of tokens 8(r/4) + 4(l/32) + r%4: a row is two lanes
+//   softmax         exp2 domain; the reference maximum follows only when a tile
+//                   passes it by 2^8, so the accumulators are seldom rescaled
+//   O^T += V^T P^T  P^T is the S^T registers, rounded to the rows' type; V^T comes
+//                   through the transpose read ds_read_b64_tr_b16.  O^T keeps a row
+//                   in its lane: rescaling and the final division stay there
+//
+// F32 rows enter as pairs of f16 terms (hi + lo, 22 bits; three products, the one
+// of two lo terms left out): v_mfma_f32_32x32x16_f16 three times does the work of
+// the fp32 form at five times its rate.  So that f16's exponents suffice for any
+// fp32 value, each row of Q, K and V is scaled by a power of two to a largest value
+// in [2^14, 2^15): Q's goes into the row's factor, K's into its token's score, V's
+// into its token's probability (kept below f16's range by a reference exponent
+// per row, as the maximum is).
+//
+// Masks are evaluated in tiles that some row of the wave does not see whole.  A
+// value that a row does not see has weight zero there, and zero times an
+// infinity or NaN must not reach the row: in tiles that some row of the workgroup
+// does not see whole, V's non-finite values are left out of the tile, and the rows
+// that do see them add them afterwards (fix_v).
+#pragma once
+
+#include "pa_common.h"
+#include "pa_launch.h"
+#include "pa_mfma.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace iian_pa {
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptThreads = kPromptWaves * 64;
+constexpr int kPromptRows = kPromptWaves * 32;   // rows per workgroup
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <int TY>
+struct PromptType;   // 1 F16, 30 BF16, 0 F32
+template <>
+struct PromptType<1> {
+    typedef _Float16 T;
+};
+template <>
+struct PromptType<30> {
+    typedef __bf16 T;
+};
+template <>
+struct PromptType<0> {
+    typedef float T;
+};
+
+// TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32; VEC: rows of
+// whole aligned 16-byte pieces.
+template <int TY, int DK, int DV>
+struct PromptShape {
+    static constexpr int NP = TY == 0 ? 2 : 1;                 // 16-bit terms per value
+    static constexpr int KT = TY == 0 || DK > 128 ? 32 : 64;   // tokens per tile
+    static constexpr int NH = KT / 32, KS = DK / 16, NO = DV / 32;
+    // rows padded by 16 bytes: 16 of them read at one offset fill the 64 banks
+    static constexpr int KSTRIDE = DK * 2 + 16;
+    // a transpose read takes 64 bytes of 4 rows: rows 16 or 48 banks apart
+    static constexpr int VSTRIDE = DV % 64 == 0 ? DV * 2 + 64 : DV * 2;
+    static constexpr int KPLANE = KT * KSTRIDE, VPLANE = KT * VSTRIDE;
+    static constexpr int KBUF = NP * KPLANE, VBUF = NP * VPLANE;
+    static constexpr int KCH = KT * (DK / 8), VCH = KT * (DV / 8);   // 8-dim pieces per tile
+    static constexpr int KPT = (KCH + kPromptThreads - 1) / kPromptThreads, VPT = (VCH + kPromptThreads - 1) / kPromptThreads;
+};
+
+template <int TY>
+struct Piece8 {   // 8 dims of one row as they are in memory
+    u32x4 a;
+};
+template <>
+struct Piece8<0> {
+    f32x4 a, b;
+};
+
+// Dims d .. d+7 of a row of D (zero past it).
+template <int TY, bool VEC>
+__device__ __forceinline__ Piece8<TY> load_piece(const typename PromptType<TY>::T *row, int d, int D, bool live) {
+    Piece8<TY> x = {};
+    if constexpr (VEC) {
+        if (live && d < D) {
+            if constexpr (TY == 0) {
+                x.a = *(const f32x4 *) (row + d);
+                x.b = *(const f32x4 *) (row + d + 4);
+            } else {
+                x.a = *(const u32x4 *) (row + d);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (live && d + e < D) {
+                if constexpr (TY == 0) {
+                    if (e < 4) x.a[e] = row[d + e];
+                    else x.b[e - 4] = row[d + e];
+                } else {
+                    const uint32_t h = ((const uint16_t *) row)[d + e];
+                    x.a[e / 2] |= h << (16 * (e & 1));
+                }
+            }
+        }
+    }
+    return x;
+}
+
+// Exponent e that scales a row's largest magnitude into [2^14, 2^15) as 2^(15 - e)
+// times it.  (At least -100, so that the factor is an ordinary number: a row of
+// zeros then never sets the reference of V's factors.)
+__device__ __forceinline__ int split_exp(float mx) {
+    return mx < INFINITY ? mx > 0.f ? max(__builtin_amdgcn_frexp_expf(mx), -100) : -100 : 15;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t) (127 + e) << 23); }
+
+// x = hi + lo to 22 bits, each rounded to nearest.  (The difference passes
+// through empty asm: folded into a mixed-precision FMA with a negated operand it
+// has come out wrong, see split_f16x8.)
+__device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16) x;
+    float f = (float) hi;
+    asm volatile("" : "+v"(f));
+    lo = (_Float16) (x - f);
+}
+
+template <int TY>
+__device__ __forceinline__ f32x16 prompt_mfma(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
+    if constexpr (TY == 30)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int TY>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (TY == 30) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const b2 v = {(__bf16) a, (__bf16) b};
+        return __builtin_bit_cast(uint32_t, v);
+    } else {
+        return pack_f16x2(a, b);
+    }
+}
+
+// Zeroes the non-finite 16-bit values of a piece; whether there were any.
+template <int TY>
+__device__ __forceinline__ bool finite_piece(Piece8<TY> &x) {
+    bool bad = false;
+    if constexpr (TY == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if ((__float_as_uint(x.a[e]) & 0x7f800000u) == 0x7f800000u) x.a[e] = 0.f, bad = true;
+            if ((__float_as_uint(x.b[e]) & 0x7f800000u) == 0x7f800000u) x.b[e] = 0.f, bad = true;
+        }
+    } else {
+        constexpr uint32_t EXP = TY == 30 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if ((x.a[i] & EXP) == EXP) x.a[i] &= 0xffff0000u, bad = true;
+            if ((x.a[i] & (EXP << 16)) == EXP << 16) x.a[i] &= 0xffffu, bad = true;
+        }
+    }
+    return bad;
+}
+
+// Row block b of the launch: the prompts' blocks in order, each prompt's last
+// (which sees the most tokens) first.  Wave-uniform; false past the last.
+__device__ __forceinline__ bool find_block(const PromptParams &p, int b, int &s, int &rb, int &q0, int &L) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int s0 = 0; s0 < p.S; s0 += 64) {
+        const int si = s0 + lane;
+        int a = 0, len = 0, n = 0;
+        if (si < p.S) {
+            a = min(max(p.qsl[si], 0), p.T);
+            len = min(max(p.qsl[si + 1], a), p.T) - a;
+            n = (int) (((int64_t) min(len, p.max_q) * p.gqa + kPromptRows - 1) / kPromptRows);
+        }
+        const int sum = wave_incl_scan(n);
+        const int total = __builtin_amdgcn_readlane(sum, 63);
+        if (b < base + total) {
+            const uint64_t m = __ballot(base + sum > b);
+            const int at = __builtin_ctzll(m);
+            s = s0 + at;
+            q0 = __builtin_amdgcn_readlane(a, at);
+            L = __builtin_amdgcn_readlane(len, at);
+            rb = base + __builtin_amdgcn_readlane(sum, at) - 1 - b;   // the last block first
+            return true;
+        }
+        base += total;
+    }
+    return false;
+}
+
+template <int TY, int DK, int DV, bool VEC>
+__global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt_kernel(PromptParams p) {
+    using SH = PromptShape<TY, DK, DV>;
+    using T = typename PromptType<TY>::T;
+    constexpr bool F32 = TY == 0;
+    constexpr int NP = SH::NP, KT = SH::KT, NH = SH::NH, KS = SH::KS, NO = SH::NO, NS = 16 * NH;
+    __shared__ __attribute__((aligned(16))) char lds_k[2][SH::KBUF];
+    __shared__ __attribute__((aligned(16))) char lds_v[2][SH::VBUF];
+    __shared__ __attribute__((aligned(16))) float k_up[2][F32 ? KT : 1];   // F32: 2^(e - 15) of each K row
+    __shared__ __attribute__((aligned(16))) float v_up[2][F32 ? KT : 1];   // and of each V row
+    // tile i had non-finite values of V (left out of it): [i % 4], set while tile i - 1
+    // is computed, read with tile i, cleared during tile i + 1
+    __shared__ int bad_v[4];
+    __shared__ int wave_end[kPromptWaves];
+
+    const int hk = blockIdx.x % p.Hkv;
+    int s, rb, q0, L;
+    if (!find_block(p, blockIdx.x / p.Hkv, s, rb, q0, L)) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
+    if (rb == 0 && hk == 0 && tid == 0 && L > p.max_q && p.err) atomicOr(p.err, 4);
+    const int rows = min(L, p.max_q) * p.gqa;   // (the host holds tokens times heads below 2^31)
+    const int wg0 = rb * kPromptRows, row0 = wg0 + 32 * wave;
+
+    // ---- the wave's rows: token i of the lane's row, and the tokens it sees, [lo, end) ----
+    const int row = row0 + n;
+    const bool live = row < rows;
+    const int i = live ? row / p.gqa : 0, head = hk * p.gqa + (live ? row - i * p.gqa : 0);
+    const int64_t t = q0 + i;
+    int end = 0;
+    if (live) end = p.row_end ? min(max(p.row_end[t], 0), L) : p.causal ? i + 1 : L;
+    const int lo = p.n_swa > 0 ? max(0, i - p.n_swa + 1) : 0;
+    // of the wave: the tokens that all of its rows see, [w_lo_all, w_end_all), and that any sees, [w_lo, w_end)
+    const int last = min(row0 + 31, rows - 1), i_first = row0 / p.gqa, i_last = last / p.gqa;
+    int w_end, w_end_all;
+    const bool w_live = row0 < rows;
+    if (p.row_end) {
+        int mx = end, mn = live ? end : INT32_MAX;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            mx = max(mx, __shfl_xor(mx, o));
+            mn = min(mn, __shfl_xor(mn, o));
+        }
+        w_end = __builtin_amdgcn_readfirstlane(mx);
+        w_end_all = __builtin_amdgcn_readfirstlane(mn);
+    } else {
+        w_end = !w_live ? 0 : p.causal ? i_last + 1 : L;
+        w_end_all = p.causal ? i_first + 1 : L;
+    }
+    const int w_lo = p.n_swa > 0 ? max(0, i_first - p.n_swa + 1) : 0;
+    const int w_lo_all = p.n_swa > 0 ? max(0, i_last - p.n_swa + 1) : 0;
+    // of the workgroup: its tiles, and the tokens that all of its rows see
+    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + kPromptRows, rows) - 1) / p.gqa;
+    int g_end, g_end_all;
+    if (p.row_end) {
+        if (lane == 0) wave_end[wave] = w_end;
+        __syncthreads();
+        g_end = 0;
+#pragma unroll
+        for (int w = 0; w < kPromptWaves; w++) g_end = max(g_end, wave_end[w]);
+        g_end = __builtin_amdgcn_readfirstlane(g_end);
+        g_end_all = 0;   // every tile may hide something from someone
+    } else {
+        g_end = p.causal ? g_last + 1 : L;
+        g_end_all = p.causal ? g_first + 1 : L;
+    }
+    const int g_lo = (p.n_swa > 0 ? max(0, g_first - p.n_swa + 1) : 0) / KT * KT;
+    const int g_lo_all = p.n_swa > 0 ? max(0, g_last - p.n_swa + 1) : 0;
+
+    // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row ----
+    u32x4 qr[NP][KS];
+    float cs = p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e;   // multiplies the product
+    {
+        const T *qp = (const T *) p.q + t * p.q_stride + (int64_t) head * p.D;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int k = 0; k < KS; k++) qr[0][k] = load_piece<TY, VEC>(qp, 16 * k + 8 * h, p.D, live).a;
+        } else {
+            Piece8<0> x[KS];
+            float mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                x[k] = load_piece<TY, VEC>(qp, 16 * k + 8 * h, p.D, live);
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(x[k].a[e]), fabsf(x[k].b[e])));
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const int ex = split_exp(mx);
+            const float up = pow2(15 - ex);
+            cs *= pow2(ex - 15);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                f16x8 hi, lw;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    _Float16 a, b;
+                    split2((e < 4 ? x[k].a[e] : x[k].b[e - 4]) * up, a, b);
+                    hi[e] = a;
+                    lw[e] = b;
+                }
+                qr[0][k] = __builtin_bit_cast(u32x4, hi);
+                qr[NP - 1][k] = __builtin_bit_cast(u32x4, lw);
+            }
+        }
+    }
+
+    // ---- staging: piece (token, 8 dims) x of a tile per thread and step ----
+    Piece8<TY> ks[SH::KPT], vs[SH::VPT];
+    const T *kb = (const T *) p.k + q0 * p.k_stride + (int64_t) hk * p.D;
+    const T *vb = (const T *) p.v + q0 * p.v_stride + (int64_t) hk * p.Dv;
+    auto load_tile = [&](int c0) {
+#pragma unroll
+        for (int x = 0; x < SH::KPT; x++) {
+            const int id = tid + x * kPromptThreads, r = id / (DK / 8), d = id % (DK / 8) * 8, j = c0 + r;
+            ks[x] = load_piece<TY, VEC>(kb + j * p.k_stride, d, p.D, id < SH::KCH && j < L);
+        }
+#pragma unroll
+        for (int x = 0; x < SH::VPT; x++) {
+            const int id = tid + x * kPromptThreads, r = id / (DV / 8), d = id % (DV / 8) * 8, j = c0 + r;
+            vs[x] = load_piece<TY, VEC>(vb + j * p.v_stride, d, p.Dv, id < SH::VCH && j < L);
+        }
+    };
+    auto put_piece = [&](const Piece8<TY> &x, char *at, int plane, float up) {
+        if constexpr (F32) {
+            f16x8 hi, lw;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                _Float16 a, b;
+                split2((e < 4 ? x.a[e] : x.b[e - 4]) * up, a, b);
+                hi[e] = a;
+                lw[e] = b;
+            }
+            *(f16x8 *) at = hi;
+            *(f16x8 *) (at + plane) = lw;
+        } else {
+            *(u32x4 *) at = x.a;
+        }
+    };
+    // Largest magnitude of the row that piece x (8 of `dims` dims, in `dims / 8`
+    // neighbouring lanes, a power of two of them) belongs to.
+    auto group_max = [&](const Piece8<TY> &x, auto dims) {
+        constexpr int G = decltype(dims)::value / 8;
+        float m = 0.f;
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+            static_assert((G & (G - 1)) == 0 && G <= 32, "rows of a power of two of pieces");
+#pragma unroll
+            for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        }
+        return m;
+    };
+    auto put_tile = [&](int c0, int buf, int idx) {
+        // (workgroup-uniform) some row of the workgroup does not see all of the tile
+        const bool part = c0 < g_lo_all || c0 + KT > g_end_all;
+#pragma unroll
+        for (int x = 0; x < SH::KPT; x++) {
+            const int id = tid + x * kPromptThreads, r = id / (DK / 8), c = id % (DK / 8);
+            float up = 1.f;
+            if constexpr (F32) {
+                const int ex = split_exp(group_max(ks[x], std::integral_constant<int, DK>()));
+                up = pow2(15 - ex);
+                if (c == 0 && id < SH::KCH) k_up[buf][r] = pow2(ex - 15);
+            }
+            if (id < SH::KCH) put_piece(ks[x], lds_k[buf] + r * SH::KSTRIDE + c * 16, SH::KPLANE, up);
+        }
+        bool bad = false;
+#pragma unroll
+        for (int x = 0; x < SH::VPT; x++) {
+            const int id = tid + x * kPromptThreads, r = id / (DV / 8), c = id % (DV / 8);
+            if (part) bad |= finite_piece<TY>(vs[x]);
+            float up = 1.f;
+            if constexpr (F32) {
+                const int ex = split_exp(group_max(vs[x], std::integral_constant<int, DV>()));
+                up = pow2(15 - ex);
+                if (c == 0 && id < SH::VCH) v_up[buf][r] = pow2(ex - 15);
+            }
+            if (id < SH::VCH) put_piece(vs[x], lds_v[buf] + r * SH::VSTRIDE + c * 16, SH::VPLANE, up);
+        }
+        if (bad) bad_v[idx & 3] = 1;
+    };
+
+    f32x16 o[NO];
+#pragma unroll
+    for (int m = 0; m < NO; m++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[m][r] = 0.f;
+    float m_ref = -INFINITY, l = 0.f;   // reference maximum (log2 units) and the lane's part of the sum
+    float v_ref = 0x1p-126f;            // F32: power of two that V's factors are taken relative to
+    if (tid < 4) bad_v[tid] = 0;
+    __syncthreads();
+
+    // lane's LDS byte offsets: K row n, dims 8h; V transpose reads: rows 4h + (lane%16)/4, dims 16((lane/16)%2) + 4(lane%4)
+    const uint32_t ka = lds_addr(lds_k[0]) + n * SH::KSTRIDE + 16 * h;
+    const uint32_t va = lds_addr(lds_v[0]) + (4 * h + ((lane & 15) >> 2)) * SH::VSTRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+
+    if (g_lo < g_end) {
+        load_tile(g_lo);
+        put_tile(g_lo, 0, 0);
+    }
+    __syncthreads();
+    int buf = 0, idx = 0;   // of the tile
+    for (int c0 = g_lo; c0 < g_end; c0 += KT, buf ^= 1, idx++) {
+        if (tid == 0) bad_v[(idx + 3) & 3] = 0;
+        const bool more = c0 + KT < g_end;
+        if (more) load_tile(c0 + KT);
+        if (c0 < w_end && c0 + KT > w_lo) {   // wave-uniform: some row sees some of the tile
+            // ---- scores ----
+            f32x16 sc[NH];
+#pragma unroll
+            for (int hh = 0; hh < NH; hh++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
+            const uint32_t kt = opaque(ka + buf * SH::KBUF);
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int hh = 0; hh < NH; hh++) {
+                    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+                    const u32x4 a = *(const lds_u32x4 *) (uintptr_t) (kt + hh * 32 * SH::KSTRIDE + 32 * k);
+                    sc[hh] = prompt_mfma<TY>(a, qr[0][k], sc[hh]);
+                    if constexpr (F32) {
+                        const u32x4 b = *(const lds_u32x4 *) (uintptr_t) (kt + SH::KPLANE + hh * 32 * SH::KSTRIDE + 32 * k);
+                        sc[hh] = prompt_mfma<TY>(b, qr[0][k], sc[hh]);
+                        sc[hh] = prompt_mfma<TY>(a, qr[NP - 1][k], sc[hh]);
+                    }
+                }
+            // ---- softmax ----
+            float x[NS];
+#pragma unroll
+            for (int j = 0; j < NS; j++) {
+                x[j] = sc[j / 16][j % 16] * cs;
+                if constexpr (F32) x[j] *= k_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
+            }
+            if (p.softcap > 0.f) {
+                const float cap = p.softcap * kLog2e;
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    if constexpr (F32) x[j] = tanhf(x[j]) * cap;
+                    else x[j] = cap - 2.f * cap / (1.f + __builtin_amdgcn_exp2f(x[j] * (2.f * kLog2e)));
+                }
+            }
+            if (c0 < w_lo_all || c0 + KT > w_end_all) {   // wave-uniform
+                const int a = lo - c0 - 4 * h, b = end - c0 - 4 * h;
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    const int key = (j / 16) * 32 + 8 * (j % 16 / 4) + j % 4;
+                    x[j] = key >= a && key < b ? x[j] : -INFINITY;
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int j = 1; j < NS; j++) mx = fmaxf(mx, x[j]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (__any(mx > m_ref + kRescaleSlack)) {
+                const float mn = mx > m_ref + kRescaleSlack ? mx : m_ref;
+                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - mn);
+                m_ref = mn;
+                l *= alpha;
+#pragma unroll
+                for (int m = 0; m < NO; m++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[m][r] *= alpha;
+            }
+            const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+            for (int j = 0; j < NS; j++) {
+                x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+                l += x[j];
+            }
+            u32x4 pr[NP][NS / 8];
+            if constexpr (F32) {
+                // V's factors: of the tokens with a weight, at most 2^6 times the row's reference
+                float vf[NS], top = 0.f;
+#pragma unroll
+                for (int j = 0; j < NS; j++) {
+                    vf[j] = v_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
+                    top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
+                }
+                top = fmaxf(top, __shfl_xor(top, 32));
+                if (__any(top > v_ref * 64.f)) {
+                    const float vn = top > v_ref * 64.f ? top : v_ref;
+                    const float beta = v_ref / vn;
+                    v_ref = vn;
+#pragma unroll
+                    for (int m = 0; m < NO; m++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[m][r] *= beta;
+                }
+                const float inv = 1.f / v_ref;
+#pragma unroll
+                for (int st = 0; st < NS / 8; st++) {
+                    f16x8 hi, lw;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        _Float16 a, b;
+                        // (a token of no weight may have any factor)
+                        split2(x[8 * st + e] != 0.f ? x[8 * st + e] * (vf[8 * st + e] * inv) : 0.f, a, b);
+                        hi[e] = a;
+                        lw[e] = b;
+                    }
+                    pr[0][st] = __builtin_bit_cast(u32x4, hi);
+                    pr[NP - 1][st] = __builtin_bit_cast(u32x4, lw);
+                }
+            } else {
+#pragma unroll
+                for (int st = 0; st < NS / 8; st++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
+            }
+            // ---- O^T += V^T P^T ----
+            const uint32_t vt = opaque(va + buf * SH::VBUF);
+#pragma unroll
+            for (int st = 0; st < NS / 8; st++)
+#pragma unroll
+                for (int m = 0; m < NO; m++) {
+                    const uint32_t at = vt + 16 * st * SH::VSTRIDE + 64 * m;
+                    const u32x4 a = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(at, at + 8 * SH::VSTRIDE));
+                    o[m] = prompt_mfma<TY>(a, pr[0][st], o[m]);
+                    if constexpr (F32) {
+                        const u32x4 b = __builtin_bit_cast(
+                            u32x4, lds_tr_b16x8_at(at + SH::VPLANE, at + SH::VPLANE + 8 * SH::VSTRIDE));
+                        o[m] = prompt_mfma<TY>(b, pr[0][st], o[m]);
+                        o[m] = prompt_mfma<TY>(a, pr[NP - 1][st], o[m]);
+                    }
+                }
+            // ---- V's non-finite values, left out of the tile, for the rows that give them a weight ----
+            if (bad_v[idx & 3]) {
+                for (int key = 0; key < KT && c0 + key < L; key++) {
+                    const int at = (key / 32) * 16 + key % 32 / 8 * 4 + key % 4;   // the score's register, in half (key/4)%2
+                    float pv = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NS; j++) pv = j == at ? x[j] : pv;
+                    const float other = __shfl_xor(pv, 32);
+                    if (((key >> 2) & 1) != h) pv = other;
+                    const T *vr = vb + (int64_t) (c0 + key) * p.v_stride;
+#pragma unroll
+                    for (int m = 0; m < NO; m++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) {
+                            const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
+                            if (d < p.Dv && pv != 0.f) {
+                                const float v = (float) vr[d];
+                                if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[m][r] += pv * v;
+                            }
+                        }
+                }
+            }
+        }
+        if (more) put_tile(c0 + KT, buf ^ 1, idx + 1);
+        __syncthreads();
+    }
+
+    // ---- rows out ----
+    l += __shfl_xor(l, 32);
+    float inv = l == 0.f ? 0.f : 1.f / l;
+    if (!live) return;
+    if constexpr (F32) inv *= v_ref;   // (an empty row: 0 * 2^-126)
+    T *out = (T *) p.out + t * p.o_stride + (int64_t) head * p.Dv;
+#pragma unroll
+    for (int m = 0; m < NO; m++)
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            const int d = 32 * m + 8 * b + 4 * h;
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = o[m][4 * b + e] * inv;
+            if (VEC && d < p.Dv) {
+                if constexpr (F32) *(float4 *) (out + d) = make_float4(y[0], y[1], y[2], y[3]);
+                else *(u32x2 *) (out + d) = u32x2{pack2<TY>(y[0], y[1]), pack2<TY>(y[2], y[3])};
+            } else if (!VEC) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (d + e < p.Dv) out[d + e] = (T) y[e];
+            }
+        }
+}
+
+template <int TY, int DK, int DV>
+static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
+    // blocks of the launch: at most one more than whole ones for each prompt
+    const int64_t rows = (int64_t) p.T * p.gqa, per = ((int64_t) p.max_q * p.gqa + kPromptRows - 1) / kPromptRows;
+    const int64_t blocks = std::min(rows / kPromptRows + p.S, per * p.S) * p.Hkv;
+    if (blocks > (1 << 23)) return hipErrorInvalidValue;   // 256 threads each: a launch holds below 2^32
+    const dim3 grid((unsigned) blocks), wg(kPromptThreads);
+    if (vec) hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, true>), grid, wg, 0, stream, p);
+    else hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, false>), grid, wg, 0, stream, p);
+    return hipGetLastError();
+}
+
+// Rows of whole aligned pieces of 16 bytes.
+template <int TY>
+static bool prompt_vec(const PromptParams &p) {
+    const int64_t es = TY == 0 ? 4 : 2;
+    const uintptr_t al = (uintptr_t) p.q | (uintptr_t) p.k | (uintptr_t) p.v | (uintptr_t) p.out;
+    return al % 16 == 0 && ((p.q_stride | p.k_stride | p.v_stride | p.o_stride) * es) % 16 == 0 && p.D % 8 == 0 && p.Dv % 8 == 0;
+}
+
+}  // namespace iian_pa
