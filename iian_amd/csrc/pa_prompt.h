@@ -63,21 +63,27 @@ struct PromptType<0> {
     typedef float T;
 };
 
-// TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32; VEC: rows of
-// whole aligned 16-byte pieces.
+// TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32.
+//
+// LDS tiles.  Rows are unpadded, so that tiles of 16-bit rows can be loaded
+// straight into LDS (16 consecutive bytes per lane), and the 16-byte pieces of
+// row r are permuted by an exclusive or with swz(r) instead: 16 rows read at one
+// piece, as QK^T does, and the 4 rows x 64 bytes of a transpose read each fill
+// the 64 banks.
 template <int TY, int DK, int DV>
 struct PromptShape {
     static constexpr int NP = TY == 0 ? 2 : 1;                 // 16-bit terms per value
     static constexpr int KT = TY == 0 || DK > 128 ? 32 : 64;   // tokens per tile
     static constexpr int NH = KT / 32, KS = DK / 16, NO = DV / 32;
-    // rows padded by 16 bytes: 16 of them read at one offset fill the 64 banks
-    static constexpr int KSTRIDE = DK * 2 + 16;
-    // a transpose read takes 64 bytes of 4 rows: rows 16 or 48 banks apart
-    static constexpr int VSTRIDE = DV % 64 == 0 ? DV * 2 + 64 : DV * 2;
-    static constexpr int KPLANE = KT * KSTRIDE, VPLANE = KT * VSTRIDE;
-    static constexpr int KBUF = NP * KPLANE, VBUF = NP * VPLANE;
-    static constexpr int KCH = KT * (DK / 8), VCH = KT * (DV / 8);   // 8-dim pieces per tile
-    static constexpr int KPT = (KCH + kPromptThreads - 1) / kPromptThreads, VPT = (VCH + kPromptThreads - 1) / kPromptThreads;
+    static constexpr int CPR = DK <= 64 ? 8 : DK <= 128 ? 16 : 32;   // 16-byte pieces per row
+    static_assert((DV <= 64 ? 8 : DV <= 128 ? 16 : 32) == CPR, "K and V rows of one pitch");
+    static constexpr int STRIDE = CPR * 16;
+    static constexpr int PLANE = KT * STRIDE, BUF = NP * PLANE;
+    static constexpr int PPT = KT * CPR / kPromptThreads;      // pieces per thread and tile
+    static_assert(PPT * kPromptThreads == KT * CPR, "pieces divide evenly");
+    __device__ static __forceinline__ int swz(int r) {
+        return CPR == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+    }
 };
 
 template <int TY>
@@ -89,12 +95,14 @@ struct Piece8<0> {
     f32x4 a, b;
 };
 
-// Dims d .. d+7 of a row of D (zero past it).
-template <int TY, bool VEC>
-__device__ __forceinline__ Piece8<TY> load_piece(const typename PromptType<TY>::T *row, int d, int D, bool live) {
+// Dims d .. d+7 of a row of D.  ZERO: zero past D and where !live; else the row
+// is there and d is below D (pieces may reach past it, VEC rows excepted, whose
+// size is whole pieces).
+template <int TY, bool VEC, bool ZERO>
+__device__ __forceinline__ Piece8<TY> load_piece(const typename PromptType<TY>::T *row, int d, int D, bool live = true) {
     Piece8<TY> x = {};
     if constexpr (VEC) {
-        if (live && d < D) {
+        if (!ZERO || (live && d < D)) {
             if constexpr (TY == 0) {
                 x.a = *(const f32x4 *) (row + d);
                 x.b = *(const f32x4 *) (row + d + 4);
@@ -105,14 +113,14 @@ __device__ __forceinline__ Piece8<TY> load_piece(const typename PromptType<TY>::
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            if (live && d + e < D) {
-                if constexpr (TY == 0) {
-                    if (e < 4) x.a[e] = row[d + e];
-                    else x.b[e - 4] = row[d + e];
-                } else {
-                    const uint32_t h = ((const uint16_t *) row)[d + e];
-                    x.a[e / 2] |= h << (16 * (e & 1));
-                }
+            const bool ok = d + e < D && (!ZERO || live);
+            if constexpr (TY == 0) {
+                const float v = ok ? row[d + e] : 0.f;
+                if (e < 4) x.a[e] = v;
+                else x.b[e - 4] = v;
+            } else {
+                const uint32_t v = ok ? ((const uint16_t *) row)[d + e] : 0;
+                x.a[e / 2] |= v << (16 * (e & 1));
             }
         }
     }
@@ -127,10 +135,11 @@ __device__ __forceinline__ int split_exp(float mx) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t) (127 + e) << 23); }
 
-// x = hi + lo to 22 bits, each rounded to nearest.  (The difference passes
+// x = hi + lo to 22 bits, each rounded to nearest.  (The difference's terms pass
 // through empty asm: folded into a mixed-precision FMA with a negated operand it
 // has come out wrong, see split_f16x8.)
 __device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
+    asm volatile("" : "+v"(x));
     hi = (_Float16) x;
     float f = (float) hi;
     asm volatile("" : "+v"(f));
@@ -145,14 +154,28 @@ __device__ __forceinline__ f32x16 prompt_mfma(const u32x4 &a, const u32x4 &b, co
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Two values rounded to nearest, in one instruction.
 template <int TY>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
     if constexpr (TY == 30) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-        const b2 v = {(__bf16) a, (__bf16) b};
-        return __builtin_bit_cast(uint32_t, v);
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
     } else {
-        return pack_f16x2(a, b);
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, h2));
+    }
+}
+
+// c plus both 16-bit values of x.
+template <int TY>
+__device__ __forceinline__ float sum2(uint32_t x, float c) {
+    if constexpr (TY == 30) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), (b2){(__bf16) 1.f, (__bf16) 1.f}, c, false);
+    } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), (h2){(_Float16) 1.f, (_Float16) 1.f}, c, false);
     }
 }
 
@@ -210,16 +233,16 @@ template <int TY, int DK, int DV, bool VEC>
 __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt_kernel(PromptParams p) {
     using SH = PromptShape<TY, DK, DV>;
     using T = typename PromptType<TY>::T;
-    constexpr bool F32 = TY == 0;
-    constexpr int NP = SH::NP, KT = SH::KT, NH = SH::NH, KS = SH::KS, NO = SH::NO, NS = 16 * NH;
-    __shared__ __attribute__((aligned(16))) char lds_k[2][SH::KBUF];
-    __shared__ __attribute__((aligned(16))) char lds_v[2][SH::VBUF];
+    constexpr bool F32 = TY == 0, DMA = VEC && !F32;   // 16-bit tiles go straight into LDS
+    constexpr int NP = SH::NP, KT = SH::KT, NH = SH::NH, KS = SH::KS, NO = SH::NO, NS = 16 * NH, CPR = SH::CPR;
+    __shared__ __attribute__((aligned(16))) char lds_k[2][SH::BUF];
+    __shared__ __attribute__((aligned(16))) char lds_v[2][SH::BUF];
     __shared__ __attribute__((aligned(16))) float k_up[2][F32 ? KT : 1];   // F32: 2^(e - 15) of each K row
     __shared__ __attribute__((aligned(16))) float v_up[2][F32 ? KT : 1];   // and of each V row
-    // tile i had non-finite values of V (left out of it): [i % 4], set while tile i - 1
-    // is computed, read with tile i, cleared during tile i + 1
+    // tile i had non-finite values of V (left out of it): [i % 4], set before tile i is
+    // computed (or while tile i - 1 is), cleared during tile i + 1
     __shared__ int bad_v[4];
-    __shared__ int wave_end[kPromptWaves];
+    __shared__ int wave_end[2][kPromptWaves];
 
     const int hk = blockIdx.x % p.Hkv;
     int s, rb, q0, L;
@@ -239,8 +262,9 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
     const int lo = p.n_swa > 0 ? max(0, i - p.n_swa + 1) : 0;
     // of the wave: the tokens that all of its rows see, [w_lo_all, w_end_all), and that any sees, [w_lo, w_end)
     const int last = min(row0 + 31, rows - 1), i_first = row0 / p.gqa, i_last = last / p.gqa;
-    int w_end, w_end_all;
-    const bool w_live = row0 < rows;
+    // of the workgroup: its tiles start in [g_lo, g_end), and all of its rows see [g_lo_all, g_end_all)
+    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + kPromptRows, rows) - 1) / p.gqa;
+    int w_end, w_end_all, g_end, g_end_all;
     if (p.row_end) {
         int mx = end, mn = live ? end : INT32_MAX;
 #pragma unroll
@@ -250,50 +274,129 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
         }
         w_end = __builtin_amdgcn_readfirstlane(mx);
         w_end_all = __builtin_amdgcn_readfirstlane(mn);
-    } else {
-        w_end = !w_live ? 0 : p.causal ? i_last + 1 : L;
-        w_end_all = p.causal ? i_first + 1 : L;
-    }
-    const int w_lo = p.n_swa > 0 ? max(0, i_first - p.n_swa + 1) : 0;
-    const int w_lo_all = p.n_swa > 0 ? max(0, i_last - p.n_swa + 1) : 0;
-    // of the workgroup: its tiles, and the tokens that all of its rows see
-    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + kPromptRows, rows) - 1) / p.gqa;
-    int g_end, g_end_all;
-    if (p.row_end) {
-        if (lane == 0) wave_end[wave] = w_end;
+        if (lane == 0) wave_end[0][wave] = mx, wave_end[1][wave] = mn;
         __syncthreads();
-        g_end = 0;
+        mx = 0, mn = INT32_MAX;
 #pragma unroll
-        for (int w = 0; w < kPromptWaves; w++) g_end = max(g_end, wave_end[w]);
-        g_end = __builtin_amdgcn_readfirstlane(g_end);
-        g_end_all = 0;   // every tile may hide something from someone
+        for (int w = 0; w < kPromptWaves; w++) mx = max(mx, wave_end[0][w]), mn = min(mn, wave_end[1][w]);
+        g_end = __builtin_amdgcn_readfirstlane(mx);
+        g_end_all = __builtin_amdgcn_readfirstlane(mn);
     } else {
+        w_end = row0 >= rows ? 0 : p.causal ? i_last + 1 : L;
+        w_end_all = p.causal ? i_first + 1 : L;
         g_end = p.causal ? g_last + 1 : L;
         g_end_all = p.causal ? g_first + 1 : L;
     }
+    const int w_lo = p.n_swa > 0 ? max(0, i_first - p.n_swa + 1) : 0;
+    const int w_lo_all = p.n_swa > 0 ? max(0, i_last - p.n_swa + 1) : 0;
     const int g_lo = (p.n_swa > 0 ? max(0, g_first - p.n_swa + 1) : 0) / KT * KT;
     const int g_lo_all = p.n_swa > 0 ? max(0, g_last - p.n_swa + 1) : 0;
 
-    // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row ----
+    // ---- staging: piece (row r, 8 dims) of a tile per thread and step; rows past the prompt's end
+    // are its last one again, dims past the head's its last ones (never seen, never stored) ----
+    const T *kb = (const T *) p.k + q0 * p.k_stride + (int64_t) hk * p.D;
+    const T *vb = (const T *) p.v + q0 * p.v_stride + (int64_t) hk * p.Dv;
+    const int pr0 = tid / CPR;   // a thread's pieces: rows pr0 + x * (threads / CPR), at one place of the row
+    auto piece_row = [&](int x) { return pr0 + x * (kPromptThreads / CPR); };
+    auto piece_dim = [&](int x, int D) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
+    const uint32_t lk0 = lds_addr(lds_k[0]), lv0 = lds_addr(lds_v[0]);
+    Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
+    auto load_tile = [&](int c0, int buf) {
+#pragma unroll
+        for (int x = 0; x < SH::PPT; x++) {
+            const int64_t j = min(c0 + piece_row(x), L - 1);
+            const T *kr = kb + j * p.k_stride, *vr = vb + j * p.v_stride;
+            if constexpr (DMA) {
+                const uint32_t at = buf * SH::BUF + (wave + x * kPromptWaves) * 1024;
+                lds_load16(kr + piece_dim(x, p.D), __builtin_amdgcn_readfirstlane(lk0 + at));
+                lds_load16(vr + piece_dim(x, p.Dv), __builtin_amdgcn_readfirstlane(lv0 + at));
+            } else {
+                ks[x] = load_piece<TY, VEC, false>(kr, piece_dim(x, p.D), p.D);
+                vs[x] = load_piece<TY, VEC, false>(vr, piece_dim(x, p.Dv), p.Dv);
+            }
+        }
+    };
+    // F32: the scale of a row's pieces, which are in CPR neighbouring lanes
+    auto row_scale = [&](const Piece8<TY> &x, float *up) {
+        float m = 0.f;
+        if constexpr (F32) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+#pragma unroll
+            for (int o = 1; o < CPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+        }
+        const int ex = split_exp(m);
+        if (tid % CPR == 0) *up = pow2(ex - 15);
+        return pow2(15 - ex);
+    };
+    auto put_piece = [&](const Piece8<TY> &x, char *at, float up) {
+        if constexpr (F32) {
+            f16x8 hi, lw;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                _Float16 a, b;
+                split2((e < 4 ? x.a[e] : x.b[e - 4]) * up, a, b);
+                hi[e] = a;
+                lw[e] = b;
+            }
+            *(f16x8 *) at = hi;
+            *(f16x8 *) (at + SH::PLANE) = lw;
+        } else {
+            *(u32x4 *) at = x.a;
+        }
+    };
+    // (workgroup-uniform) some row of the workgroup does not see all of the tile
+    auto partial = [&](int c0) { return c0 < g_lo_all || c0 + KT > g_end_all; };
+    auto put_tile = [&](int c0, int buf, int idx) {
+        if constexpr (!DMA) {
+            bool bad = false;
+#pragma unroll
+            for (int x = 0; x < SH::PPT; x++) {
+                const int at = (tid + x * kPromptThreads) * 16, r = piece_row(x);
+                float up = 1.f;
+                if constexpr (F32) up = row_scale(ks[x], &k_up[buf][r]);
+                put_piece(ks[x], lds_k[buf] + at, up);
+                if (partial(c0)) bad |= finite_piece<TY>(vs[x]);
+                if constexpr (F32) up = row_scale(vs[x], &v_up[buf][r]);
+                put_piece(vs[x], lds_v[buf] + at, up);
+            }
+            if (bad) bad_v[idx & 3] = 1;
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+    };
+
+    // the first tile is on its way while Q is loaded
+    if (tid < 4) bad_v[tid] = 0;
+    if constexpr (!DMA) __syncthreads();
+    if (g_lo < g_end) load_tile(g_lo, 0);
+
+    // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
     u32x4 qr[NP][KS];
-    float cs = p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e;   // multiplies the product
+    // of the product; above zero, so that a masked score stays -inf (a scale of zero takes Q as zero instead)
+    float cs = p.scale == 0.f ? 1.f : fabsf(p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e);
     {
         const T *qp = (const T *) p.q + t * p.q_stride + (int64_t) head * p.D;
         if constexpr (!F32) {
+            const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0;
 #pragma unroll
-            for (int k = 0; k < KS; k++) qr[0][k] = load_piece<TY, VEC>(qp, 16 * k + 8 * h, p.D, live).a;
+            for (int k = 0; k < KS; k++) {
+                qr[0][k] = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live).a;
+#pragma unroll
+                for (int e = 0; e < 4; e++) qr[0][k][e] = p.scale == 0.f ? 0 : qr[0][k][e] ^ sign;
+            }
         } else {
             Piece8<0> x[KS];
             float mx = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                x[k] = load_piece<TY, VEC>(qp, 16 * k + 8 * h, p.D, live);
+                x[k] = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live);
 #pragma unroll
                 for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(x[k].a[e]), fabsf(x[k].b[e])));
             }
             mx = fmaxf(mx, __shfl_xor(mx, 32));
             const int ex = split_exp(mx);
-            const float up = pow2(15 - ex);
+            const float up = p.scale == 0.f ? 0.f : p.scale < 0.f ? -pow2(15 - ex) : pow2(15 - ex);
             cs *= pow2(ex - 15);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
@@ -309,83 +412,14 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
                 qr[NP - 1][k] = __builtin_bit_cast(u32x4, lw);
             }
         }
+        cs = fmaxf(cs, 1e-37f);
+        // Q is here: no wait for it (and with it for the tile in flight) inside the loop
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            asm volatile("" : "+v"(qr[0][k]));
+            if constexpr (F32) asm volatile("" : "+v"(qr[NP - 1][k]));
+        }
     }
-
-    // ---- staging: piece (token, 8 dims) x of a tile per thread and step ----
-    Piece8<TY> ks[SH::KPT], vs[SH::VPT];
-    const T *kb = (const T *) p.k + q0 * p.k_stride + (int64_t) hk * p.D;
-    const T *vb = (const T *) p.v + q0 * p.v_stride + (int64_t) hk * p.Dv;
-    auto load_tile = [&](int c0) {
-#pragma unroll
-        for (int x = 0; x < SH::KPT; x++) {
-            const int id = tid + x * kPromptThreads, r = id / (DK / 8), d = id % (DK / 8) * 8, j = c0 + r;
-            ks[x] = load_piece<TY, VEC>(kb + j * p.k_stride, d, p.D, id < SH::KCH && j < L);
-        }
-#pragma unroll
-        for (int x = 0; x < SH::VPT; x++) {
-            const int id = tid + x * kPromptThreads, r = id / (DV / 8), d = id % (DV / 8) * 8, j = c0 + r;
-            vs[x] = load_piece<TY, VEC>(vb + j * p.v_stride, d, p.Dv, id < SH::VCH && j < L);
-        }
-    };
-    auto put_piece = [&](const Piece8<TY> &x, char *at, int plane, float up) {
-        if constexpr (F32) {
-            f16x8 hi, lw;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                _Float16 a, b;
-                split2((e < 4 ? x.a[e] : x.b[e - 4]) * up, a, b);
-                hi[e] = a;
-                lw[e] = b;
-            }
-            *(f16x8 *) at = hi;
-            *(f16x8 *) (at + plane) = lw;
-        } else {
-            *(u32x4 *) at = x.a;
-        }
-    };
-    // Largest magnitude of the row that piece x (8 of `dims` dims, in `dims / 8`
-    // neighbouring lanes, a power of two of them) belongs to.
-    auto group_max = [&](const Piece8<TY> &x, auto dims) {
-        constexpr int G = decltype(dims)::value / 8;
-        float m = 0.f;
-        if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
-            static_assert((G & (G - 1)) == 0 && G <= 32, "rows of a power of two of pieces");
-#pragma unroll
-            for (int o = 1; o < G; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        }
-        return m;
-    };
-    auto put_tile = [&](int c0, int buf, int idx) {
-        // (workgroup-uniform) some row of the workgroup does not see all of the tile
-        const bool part = c0 < g_lo_all || c0 + KT > g_end_all;
-#pragma unroll
-        for (int x = 0; x < SH::KPT; x++) {
-            const int id = tid + x * kPromptThreads, r = id / (DK / 8), c = id % (DK / 8);
-            float up = 1.f;
-            if constexpr (F32) {
-                const int ex = split_exp(group_max(ks[x], std::integral_constant<int, DK>()));
-                up = pow2(15 - ex);
-                if (c == 0 && id < SH::KCH) k_up[buf][r] = pow2(ex - 15);
-            }
-            if (id < SH::KCH) put_piece(ks[x], lds_k[buf] + r * SH::KSTRIDE + c * 16, SH::KPLANE, up);
-        }
-        bool bad = false;
-#pragma unroll
-        for (int x = 0; x < SH::VPT; x++) {
-            const int id = tid + x * kPromptThreads, r = id / (DV / 8), c = id % (DV / 8);
-            if (part) bad |= finite_piece<TY>(vs[x]);
-            float up = 1.f;
-            if constexpr (F32) {
-                const int ex = split_exp(group_max(vs[x], std::integral_constant<int, DV>()));
-                up = pow2(15 - ex);
-                if (c == 0 && id < SH::VCH) v_up[buf][r] = pow2(ex - 15);
-            }
-            if (id < SH::VCH) put_piece(vs[x], lds_v[buf] + r * SH::VSTRIDE + c * 16, SH::VPLANE, up);
-        }
-        if (bad) bad_v[idx & 3] = 1;
-    };
 
     f32x16 o[NO];
 #pragma unroll
@@ -394,58 +428,80 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
         for (int r = 0; r < 16; r++) o[m][r] = 0.f;
     float m_ref = -INFINITY, l = 0.f;   // reference maximum (log2 units) and the lane's part of the sum
     float v_ref = 0x1p-126f;            // F32: power of two that V's factors are taken relative to
-    if (tid < 4) bad_v[tid] = 0;
-    __syncthreads();
 
-    // lane's LDS byte offsets: K row n, dims 8h; V transpose reads: rows 4h + (lane%16)/4, dims 16((lane/16)%2) + 4(lane%4)
-    const uint32_t ka = lds_addr(lds_k[0]) + n * SH::KSTRIDE + 16 * h;
-    const uint32_t va = lds_addr(lds_v[0]) + (4 * h + ((lane & 15) >> 2)) * SH::VSTRIDE + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    // lane's LDS byte offsets.  K row n (+ 32 hh), piece 2k + h; V transpose reads: rows 4h + (lane%16)/4 (+ 8, + 16 st),
+    // dims 32m + 16((lane/16)%2) + 4(lane%4): piece 4m + 2((lane/16)%2) + (lane%4)/2, 8 bytes into it for odd lanes.  The
+    // exclusive or does not mix with the constants added, so a base per distinct pattern is kept: swz(n) is K's; rows r and
+    // r + 8 (r + 16 is r again) are V's.
+    const int vrow = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    uint32_t koff[KS], voff[2][NO];
+#pragma unroll
+    for (int k = 0; k < KS; k++) koff[k] = lk0 + n * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n));
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int m = 0; m < NO; m++)
+            voff[e][m] = lv0 + (vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
 
-    if (g_lo < g_end) {
-        load_tile(g_lo);
-        put_tile(g_lo, 0, 0);
-    }
+    if (g_lo < g_end) put_tile(g_lo, 0, 0);
     __syncthreads();
     int buf = 0, idx = 0;   // of the tile
     for (int c0 = g_lo; c0 < g_end; c0 += KT, buf ^= 1, idx++) {
         if (tid == 0) bad_v[(idx + 3) & 3] = 0;
         const bool more = c0 + KT < g_end;
-        if (more) load_tile(c0 + KT);
+        if (more) load_tile(c0 + KT, buf ^ 1);
+        if (DMA && partial(c0)) {
+            bool bad = false;
+#pragma unroll
+            for (int x = 0; x < SH::PPT; x++) {
+                Piece8<TY> v;
+                u32x4 *at = (u32x4 *) (lds_v[buf] + (tid + x * kPromptThreads) * 16);
+                if constexpr (!F32) {
+                    v.a = *at;
+                    if (finite_piece<TY>(v)) *at = v.a, bad = true;
+                }
+            }
+            if (bad) bad_v[idx & 3] = 1;
+            __syncthreads();
+        }
         if (c0 < w_end && c0 + KT > w_lo) {   // wave-uniform: some row sees some of the tile
+            typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
             // ---- scores ----
             f32x16 sc[NH];
 #pragma unroll
             for (int hh = 0; hh < NH; hh++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
-            const uint32_t kt = opaque(ka + buf * SH::KBUF);
+            const uint32_t bo = buf * SH::BUF;
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++) {
+                const uint32_t at = koff[k] + bo;
 #pragma unroll
                 for (int hh = 0; hh < NH; hh++) {
-                    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-                    const u32x4 a = *(const lds_u32x4 *) (uintptr_t) (kt + hh * 32 * SH::KSTRIDE + 32 * k);
+                    const u32x4 a = *(const lds_u32x4 *) (uintptr_t) (at + hh * 32 * SH::STRIDE);
                     sc[hh] = prompt_mfma<TY>(a, qr[0][k], sc[hh]);
                     if constexpr (F32) {
-                        const u32x4 b = *(const lds_u32x4 *) (uintptr_t) (kt + SH::KPLANE + hh * 32 * SH::KSTRIDE + 32 * k);
+                        const u32x4 b = *(const lds_u32x4 *) (uintptr_t) (at + SH::PLANE + hh * 32 * SH::STRIDE);
                         sc[hh] = prompt_mfma<TY>(b, qr[0][k], sc[hh]);
                         sc[hh] = prompt_mfma<TY>(a, qr[NP - 1][k], sc[hh]);
                     }
                 }
+            }
             // ---- softmax ----
             float x[NS];
+            float cx = cs;   // x times cx is the score in log2 units
 #pragma unroll
             for (int j = 0; j < NS; j++) {
-                x[j] = sc[j / 16][j % 16] * cs;
+                x[j] = sc[j / 16][j % 16];
                 if constexpr (F32) x[j] *= k_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
             }
             if (p.softcap > 0.f) {
-                const float cap = p.softcap * kLog2e;
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
-                    if constexpr (F32) x[j] = tanhf(x[j]) * cap;
-                    else x[j] = cap - 2.f * cap / (1.f + __builtin_amdgcn_exp2f(x[j] * (2.f * kLog2e)));
+                    if constexpr (F32) x[j] = tanhf(x[j] * cs);
+                    else x[j] = 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x[j] * (cs * (2.f * kLog2e))));
                 }
+                cx = p.softcap * kLog2e;
             }
             if (c0 < w_lo_all || c0 + KT > w_end_all) {   // wave-uniform
                 const int a = lo - c0 - 4 * h, b = end - c0 - 4 * h;
@@ -458,7 +514,7 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
             float mx = x[0];
 #pragma unroll
             for (int j = 1; j < NS; j++) mx = fmaxf(mx, x[j]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * cx;
             if (__any(mx > m_ref + kRescaleSlack)) {
                 const float mn = mx > m_ref + kRescaleSlack ? mx : m_ref;
                 const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - mn);
@@ -471,12 +527,11 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
             }
             const float ref = m_ref == -INFINITY ? 0.f : m_ref;
 #pragma unroll
-            for (int j = 0; j < NS; j++) {
-                x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
-                l += x[j];
-            }
+            for (int j = 0; j < NS; j++) x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], cx, -ref));
             u32x4 pr[NP][NS / 8];
             if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < NS; j++) l += x[j];
                 // V's factors: of the tokens with a weight, at most 2^6 times the row's reference
                 float vf[NS], top = 0.f;
 #pragma unroll
@@ -510,45 +565,42 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
                     pr[NP - 1][st] = __builtin_bit_cast(u32x4, lw);
                 }
             } else {
+                // the sum is of the rounded probabilities, as the products are
 #pragma unroll
                 for (int st = 0; st < NS / 8; st++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
+                    for (int e = 0; e < 4; e++) {
+                        pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
+                        l = sum2<TY>(pr[0][st][e], l);
+                    }
             }
             // ---- O^T += V^T P^T ----
-            const uint32_t vt = opaque(va + buf * SH::VBUF);
 #pragma unroll
             for (int st = 0; st < NS / 8; st++)
 #pragma unroll
                 for (int m = 0; m < NO; m++) {
-                    const uint32_t at = vt + 16 * st * SH::VSTRIDE + 64 * m;
-                    const u32x4 a = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(at, at + 8 * SH::VSTRIDE));
+                    const uint32_t a0 = voff[0][m] + bo + 16 * st * SH::STRIDE, a1 = voff[1][m] + bo + 16 * st * SH::STRIDE;
+                    const u32x4 a = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(a0, a1));
                     o[m] = prompt_mfma<TY>(a, pr[0][st], o[m]);
                     if constexpr (F32) {
-                        const u32x4 b = __builtin_bit_cast(
-                            u32x4, lds_tr_b16x8_at(at + SH::VPLANE, at + SH::VPLANE + 8 * SH::VSTRIDE));
+                        const u32x4 b = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(a0 + SH::PLANE, a1 + SH::PLANE));
                         o[m] = prompt_mfma<TY>(b, pr[0][st], o[m]);
                         o[m] = prompt_mfma<TY>(a, pr[NP - 1][st], o[m]);
                     }
                 }
-            // ---- V's non-finite values, left out of the tile, for the rows that give them a weight ----
+            // ---- V's non-finite values, left out of the tile, for the rows that see them ----
             if (bad_v[idx & 3]) {
                 for (int key = 0; key < KT && c0 + key < L; key++) {
-                    const int at = (key / 32) * 16 + key % 32 / 8 * 4 + key % 4;   // the score's register, in half (key/4)%2
-                    float pv = 0.f;
-#pragma unroll
-                    for (int j = 0; j < NS; j++) pv = j == at ? x[j] : pv;
-                    const float other = __shfl_xor(pv, 32);
-                    if (((key >> 2) & 1) != h) pv = other;
+                    const bool sees = c0 + key >= lo && c0 + key < end;
                     const T *vr = vb + (int64_t) (c0 + key) * p.v_stride;
 #pragma unroll
                     for (int m = 0; m < NO; m++)
 #pragma unroll
                         for (int r = 0; r < 16; r++) {
                             const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
-                            if (d < p.Dv && pv != 0.f) {
+                            if (d < p.Dv && sees) {
                                 const float v = (float) vr[d];
-                                if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[m][r] += pv * v;
+                                if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[m][r] += v;
                             }
                         }
                 }
