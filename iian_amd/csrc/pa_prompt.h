@@ -230,7 +230,8 @@ __device__ __forceinline__ bool find_block(const PromptParams &p, int b, int &s,
 }
 
 template <int TY, int DK, int DV, bool VEC>
-__global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt_kernel(PromptParams p) {
+__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(DK <= 128 ? 2 : 1))) void
+pa_prompt_kernel(PromptParams p) {
     using SH = PromptShape<TY, DK, DV>;
     using T = typename PromptType<TY>::T;
     constexpr bool F32 = TY == 0, DMA = VEC && !F32;   // 16-bit tiles go straight into LDS
@@ -301,18 +302,39 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
     auto piece_dim = [&](int x, int D) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k[0]), lv0 = lds_addr(lds_v[0]);
     Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
-    auto load_tile = [&](int c0, int buf) {
+    // 16-bit rows: byte offsets of a thread's pieces of x = 0 and 1 (every other x has x & 1's place in its row)
+    uint32_t kvo[2], vvo[2];
+    if constexpr (DMA) {
 #pragma unroll
-        for (int x = 0; x < SH::PPT; x++) {
-            const int64_t j = min(c0 + piece_row(x), L - 1);
-            const T *kr = kb + j * p.k_stride, *vr = vb + j * p.v_stride;
-            if constexpr (DMA) {
+        for (int x = 0; x < 2; x++) {
+            kvo[x] = (pr0 * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2;
+            vvo[x] = (pr0 * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2;
+        }
+    }
+    auto load_tile = [&](int c0, int buf) {
+        if constexpr (DMA) {
+            const bool whole = c0 + KT <= L;
+#pragma unroll
+            for (int x = 0; x < SH::PPT; x++) {
+                constexpr int RPX = kPromptThreads / CPR;
                 const uint32_t at = buf * SH::BUF + (wave + x * kPromptWaves) * 1024;
-                lds_load16(kr + piece_dim(x, p.D), __builtin_amdgcn_readfirstlane(lk0 + at));
-                lds_load16(vr + piece_dim(x, p.Dv), __builtin_amdgcn_readfirstlane(lv0 + at));
-            } else {
-                ks[x] = load_piece<TY, VEC, false>(kr, piece_dim(x, p.D), p.D);
-                vs[x] = load_piece<TY, VEC, false>(vr, piece_dim(x, p.Dv), p.Dv);
+                uint32_t ko = kvo[x & 1], vo = vvo[x & 1];
+                int64_t r0 = c0 + x * RPX;
+                if (!whole) {
+                    r0 = c0;
+                    const uint32_t r = min(piece_row(x), L - 1 - c0);
+                    ko = (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2;
+                    vo = (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2;
+                }
+                lds_load16_s(kb + r0 * p.k_stride, ko, __builtin_amdgcn_readfirstlane(lk0 + at));
+                lds_load16_s(vb + r0 * p.v_stride, vo, __builtin_amdgcn_readfirstlane(lv0 + at));
+            }
+        } else {
+#pragma unroll
+            for (int x = 0; x < SH::PPT; x++) {
+                const int64_t j = min(c0 + piece_row(x), L - 1);
+                ks[x] = load_piece<TY, VEC, false>(kb + j * p.k_stride, piece_dim(x, p.D), p.D);
+                vs[x] = load_piece<TY, VEC, false>(vb + j * p.v_stride, piece_dim(x, p.Dv), p.Dv);
             }
         }
     };
@@ -473,19 +495,32 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
 #pragma unroll
                 for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
             const uint32_t bo = buf * SH::BUF;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
+            // Operands are read two products' worth ahead; the scheduling barriers keep the compiler from pulling
+            // each read down to its product, where the wave would wait for it.
+            u32x4 kr[3][NH][NP];
+            auto read_k = [&](int k) {
                 const uint32_t at = koff[k] + bo;
 #pragma unroll
+                for (int hh = 0; hh < NH; hh++)
+#pragma unroll
+                    for (int e = 0; e < NP; e++)
+                        kr[k % 3][hh][e] = *(const lds_u32x4 *) (uintptr_t) (at + e * SH::PLANE + hh * 32 * SH::STRIDE);
+            };
+            read_k(0);
+            read_k(1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                if (k + 2 < KS) read_k(k + 2);
+#pragma unroll
                 for (int hh = 0; hh < NH; hh++) {
-                    const u32x4 a = *(const lds_u32x4 *) (uintptr_t) (at + hh * 32 * SH::STRIDE);
-                    sc[hh] = prompt_mfma<TY>(a, qr[0][k], sc[hh]);
+                    sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][0], qr[0][k], sc[hh]);
                     if constexpr (F32) {
-                        const u32x4 b = *(const lds_u32x4 *) (uintptr_t) (at + SH::PLANE + hh * 32 * SH::STRIDE);
-                        sc[hh] = prompt_mfma<TY>(b, qr[0][k], sc[hh]);
-                        sc[hh] = prompt_mfma<TY>(a, qr[NP - 1][k], sc[hh]);
+                        sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][NP - 1], qr[0][k], sc[hh]);
+                        sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][0], qr[NP - 1][k], sc[hh]);
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             // ---- softmax ----
             float x[NS];
@@ -526,12 +561,13 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
                     for (int r = 0; r < 16; r++) o[m][r] *= alpha;
             }
             const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
-            for (int j = 0; j < NS; j++) x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], cx, -ref));
             u32x4 pr[NP][NS / 8];
             if constexpr (F32) {
 #pragma unroll
-                for (int j = 0; j < NS; j++) l += x[j];
+                for (int j = 0; j < NS; j++) {
+                    x[j] = __builtin_amdgcn_exp2f(fmaf(x[j], cx, -ref));
+                    l += x[j];
+                }
                 // V's factors: of the tokens with a weight, at most 2^6 times the row's reference
                 float vf[NS], top = 0.f;
 #pragma unroll
@@ -564,30 +600,46 @@ __global__ __launch_bounds__(kPromptThreads, (DK <= 128 ? 2 : 1)) void pa_prompt
                     pr[0][st] = __builtin_bit_cast(u32x4, hi);
                     pr[NP - 1][st] = __builtin_bit_cast(u32x4, lw);
                 }
-            } else {
-                // the sum is of the rounded probabilities, as the products are
-#pragma unroll
-                for (int st = 0; st < NS / 8; st++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
-                        l = sum2<TY>(pr[0][st][e], l);
-                    }
             }
-            // ---- O^T += V^T P^T ----
+            // ---- O^T += V^T P^T, the next 16 tokens' probabilities beside the products of 16 ----
+            // (the sum is of the rounded probabilities, as the products are)
+            auto weigh = [&](int st, int e) {   // pair e of the 16 tokens st
+                x[8 * st + 2 * e] = __builtin_amdgcn_exp2f(fmaf(x[8 * st + 2 * e], cx, -ref));
+                x[8 * st + 2 * e + 1] = __builtin_amdgcn_exp2f(fmaf(x[8 * st + 2 * e + 1], cx, -ref));
+                pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
+                l = sum2<TY>(pr[0][st][e], l);
+            };
+            constexpr int NQ = NO * (NS / 8);   // products (triples of them, F32)
+            u32x4 vr[3][NP];
+            auto read_v = [&](int q) {
+                const int st = q / NO, m = q % NO;
 #pragma unroll
-            for (int st = 0; st < NS / 8; st++)
-#pragma unroll
-                for (int m = 0; m < NO; m++) {
-                    const uint32_t a0 = voff[0][m] + bo + 16 * st * SH::STRIDE, a1 = voff[1][m] + bo + 16 * st * SH::STRIDE;
-                    const u32x4 a = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(a0, a1));
-                    o[m] = prompt_mfma<TY>(a, pr[0][st], o[m]);
-                    if constexpr (F32) {
-                        const u32x4 b = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(a0 + SH::PLANE, a1 + SH::PLANE));
-                        o[m] = prompt_mfma<TY>(b, pr[0][st], o[m]);
-                        o[m] = prompt_mfma<TY>(a, pr[NP - 1][st], o[m]);
-                    }
+                for (int e = 0; e < NP; e++) {
+                    const uint32_t off = bo + e * SH::PLANE + 16 * st * SH::STRIDE;
+                    vr[q % 3][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
                 }
+            };
+            read_v(0);
+            read_v(1);
+            if constexpr (!F32) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) weigh(0, e);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+                const int st = q / NO, m = q % NO;
+                if (q + 2 < NQ) read_v(q + 2);
+                o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[0][st], o[m]);
+                if constexpr (F32) {
+                    o[m] = prompt_mfma<TY>(vr[q % 3][NP - 1], pr[0][st], o[m]);
+                    o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[NP - 1][st], o[m]);
+                } else if (st + 1 < NS / 8) {
+#pragma unroll
+                    for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             // ---- V's non-finite values, left out of the tile, for the rows that see them ----
             if (bad_v[idx & 3]) {
                 for (int key = 0; key < KT && c0 + key < L; key++) {
@@ -652,6 +704,8 @@ template <int TY>
 static bool prompt_vec(const PromptParams &p) {
     const int64_t es = TY == 0 ? 4 : 2;
     const uintptr_t al = (uintptr_t) p.q | (uintptr_t) p.k | (uintptr_t) p.v | (uintptr_t) p.out;
+    // (a tile's rows are addressed by 32-bit offsets)
+    if (std::max(p.k_stride, p.v_stride) >= 1 << 24) return false;
     return al % 16 == 0 && ((p.q_stride | p.k_stride | p.v_stride | p.o_stride) * es) % 16 == 0 && p.D % 8 == 0 && p.Dv % 8 == 0;
 }
 
