@@ -127,6 +127,12 @@ __device__ __forceinline__ Piece8<TY> load_piece(const typename PromptType<TY>::
     return x;
 }
 
+// lds_load16_s at a wave-uniform LDS base plus a constant.  (A load into LDS wants one wait state behind the write of m0.)
+__device__ __forceinline__ void lds_load16_at(const void *sbase, uint32_t voff, uint32_t lds_base, int lds_off) {
+    asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_base), "v"(voff), "s"(sbase), "i"(lds_off)
+                 : "m0", "scc");
+}
+
 // Exponent e that scales a row's largest magnitude into [2^14, 2^15) as 2^(15 - e)
 // times it.  (At least -100, so that the factor is an ordinary number: a row of
 // zeros then never sets the reference of V's factors.)
@@ -177,6 +183,12 @@ __device__ __forceinline__ float sum2(uint32_t x, float c) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), (h2){(_Float16) 1.f, (_Float16) 1.f}, c, false);
     }
+}
+
+// The larger of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
 // Zeroes the non-finite 16-bit values of a piece; whether there were any.
@@ -240,9 +252,7 @@ pa_prompt_kernel(PromptParams p) {
     __shared__ __attribute__((aligned(16))) char lds_v[2][SH::BUF];
     __shared__ __attribute__((aligned(16))) float k_up[2][F32 ? KT : 1];   // F32: 2^(e - 15) of each K row
     __shared__ __attribute__((aligned(16))) float v_up[2][F32 ? KT : 1];   // and of each V row
-    // tile i had non-finite values of V (left out of it): [i % 4], set before tile i is
-    // computed (or while tile i - 1 is), cleared during tile i + 1
-    __shared__ int bad_v[4];
+    __shared__ int bad_v;   // some tile that is not seen whole had non-finite values of V (left out of it)
     __shared__ int wave_end[2][kPromptWaves];
 
     const int hk = blockIdx.x % p.Hkv;
@@ -302,32 +312,33 @@ pa_prompt_kernel(PromptParams p) {
     auto piece_dim = [&](int x, int D) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k[0]), lv0 = lds_addr(lds_v[0]);
     Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
-    // 16-bit rows: byte offsets of a thread's pieces of x = 0 and 1 (every other x has x & 1's place in its row)
-    uint32_t kvo[2], vvo[2];
+    // 16-bit rows: byte offsets of a thread's pieces from the tile's first row
+    uint32_t kvo[SH::PPT], vvo[SH::PPT];
     if constexpr (DMA) {
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-            kvo[x] = (pr0 * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2;
-            vvo[x] = (pr0 * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2;
+        for (int x = 0; x < SH::PPT; x++) {
+            kvo[x] = (piece_row(x) * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2;
+            vvo[x] = (piece_row(x) * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2;
         }
     }
+    const uint32_t lkw = __builtin_amdgcn_readfirstlane(lk0 + wave * 1024), lvw = __builtin_amdgcn_readfirstlane(lv0 + wave * 1024);
     auto load_tile = [&](int c0, int buf) {
         if constexpr (DMA) {
-            const bool whole = c0 + KT <= L;
+            const T *kt = kb + c0 * p.k_stride, *vt = vb + c0 * p.v_stride;
+            const uint32_t ka = lkw + buf * SH::BUF, va = lvw + buf * SH::BUF;
+            if (c0 + KT <= L) {
 #pragma unroll
-            for (int x = 0; x < SH::PPT; x++) {
-                constexpr int RPX = kPromptThreads / CPR;
-                const uint32_t at = buf * SH::BUF + (wave + x * kPromptWaves) * 1024;
-                uint32_t ko = kvo[x & 1], vo = vvo[x & 1];
-                int64_t r0 = c0 + x * RPX;
-                if (!whole) {
-                    r0 = c0;
-                    const uint32_t r = min(piece_row(x), L - 1 - c0);
-                    ko = (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2;
-                    vo = (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2;
+                for (int x = 0; x < SH::PPT; x++) {
+                    lds_load16_at(kt, kvo[x], ka, x * kPromptThreads * 16);
+                    lds_load16_at(vt, vvo[x], va, x * kPromptThreads * 16);
                 }
-                lds_load16_s(kb + r0 * p.k_stride, ko, __builtin_amdgcn_readfirstlane(lk0 + at));
-                lds_load16_s(vb + r0 * p.v_stride, vo, __builtin_amdgcn_readfirstlane(lv0 + at));
+            } else {
+#pragma unroll
+                for (int x = 0; x < SH::PPT; x++) {
+                    const uint32_t r = min(piece_row(x), L - 1 - c0);
+                    lds_load16_at(kt, (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2, ka, x * kPromptThreads * 16);
+                    lds_load16_at(vt, (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2, va, x * kPromptThreads * 16);
+                }
             }
         } else {
 #pragma unroll
@@ -369,7 +380,7 @@ pa_prompt_kernel(PromptParams p) {
     };
     // (workgroup-uniform) some row of the workgroup does not see all of the tile
     auto partial = [&](int c0) { return c0 < g_lo_all || c0 + KT > g_end_all; };
-    auto put_tile = [&](int c0, int buf, int idx) {
+    auto put_tile = [&](int c0, int buf) {
         if constexpr (!DMA) {
             bool bad = false;
 #pragma unroll
@@ -382,14 +393,14 @@ pa_prompt_kernel(PromptParams p) {
                 if constexpr (F32) up = row_scale(vs[x], &v_up[buf][r]);
                 put_piece(vs[x], lds_v[buf] + at, up);
             }
-            if (bad) bad_v[idx & 3] = 1;
+            if (bad) bad_v = 1;
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
 
     // the first tile is on its way while Q is loaded
-    if (tid < 4) bad_v[tid] = 0;
+    if (tid == 0) bad_v = 0;
     if constexpr (!DMA) __syncthreads();
     if (g_lo < g_end) load_tile(g_lo, 0);
 
@@ -448,7 +459,7 @@ pa_prompt_kernel(PromptParams p) {
     for (int m = 0; m < NO; m++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[m][r] = 0.f;
-    float m_ref = -INFINITY, l = 0.f;   // reference maximum (log2 units) and the lane's part of the sum
+    float m_ref = -0x1p127f, l = 0.f;   // reference maximum (log2 units, below any score) and the lane's part of the sum
     float v_ref = 0x1p-126f;            // F32: power of two that V's factors are taken relative to
 
     // lane's LDS byte offsets.  K row n (+ 32 hh), piece 2k + h; V transpose reads: rows 4h + (lane%16)/4 (+ 8, + 16 st),
@@ -465,11 +476,10 @@ pa_prompt_kernel(PromptParams p) {
         for (int m = 0; m < NO; m++)
             voff[e][m] = lv0 + (vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
 
-    if (g_lo < g_end) put_tile(g_lo, 0, 0);
+    if (g_lo < g_end) put_tile(g_lo, 0);
     __syncthreads();
-    int buf = 0, idx = 0;   // of the tile
-    for (int c0 = g_lo; c0 < g_end; c0 += KT, buf ^= 1, idx++) {
-        if (tid == 0) bad_v[(idx + 3) & 3] = 0;
+    int buf = 0;
+    for (int c0 = g_lo; c0 < g_end; c0 += KT, buf ^= 1) {
         const bool more = c0 + KT < g_end;
         if (more) load_tile(c0 + KT, buf ^ 1);
         if (DMA && partial(c0)) {
@@ -483,7 +493,7 @@ pa_prompt_kernel(PromptParams p) {
                     if (finite_piece<TY>(v)) *at = v.a, bad = true;
                 }
             }
-            if (bad) bad_v[idx & 3] = 1;
+            if (bad) bad_v = 1;
             __syncthreads();
         }
         if (c0 < w_end && c0 + KT > w_lo) {   // wave-uniform: some row sees some of the tile
@@ -549,10 +559,10 @@ pa_prompt_kernel(PromptParams p) {
             float mx = x[0];
 #pragma unroll
             for (int j = 1; j < NS; j++) mx = fmaxf(mx, x[j]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * cx;
+            mx = max_halves(mx) * cx;
             if (__any(mx > m_ref + kRescaleSlack)) {
                 const float mn = mx > m_ref + kRescaleSlack ? mx : m_ref;
-                const float alpha = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m_ref - mn);
+                const float alpha = __builtin_amdgcn_exp2f(m_ref - mn);
                 m_ref = mn;
                 l *= alpha;
 #pragma unroll
@@ -560,7 +570,7 @@ pa_prompt_kernel(PromptParams p) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) o[m][r] *= alpha;
             }
-            const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+            const float ref = m_ref;
             u32x4 pr[NP][NS / 8];
             if constexpr (F32) {
 #pragma unroll
@@ -575,7 +585,7 @@ pa_prompt_kernel(PromptParams p) {
                     vf[j] = v_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
                     top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
                 }
-                top = fmaxf(top, __shfl_xor(top, 32));
+                top = max_halves(top);
                 if (__any(top > v_ref * 64.f)) {
                     const float vn = top > v_ref * 64.f ? top : v_ref;
                     const float beta = v_ref / vn;
@@ -640,27 +650,26 @@ pa_prompt_kernel(PromptParams p) {
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            // ---- V's non-finite values, left out of the tile, for the rows that see them ----
-            if (bad_v[idx & 3]) {
-                for (int key = 0; key < KT && c0 + key < L; key++) {
-                    const bool sees = c0 + key >= lo && c0 + key < end;
-                    const T *vr = vb + (int64_t) (c0 + key) * p.v_stride;
-#pragma unroll
-                    for (int m = 0; m < NO; m++)
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
-                            if (d < p.Dv && sees) {
-                                const float v = (float) vr[d];
-                                if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) o[m][r] += v;
-                            }
-                        }
-                }
-            }
         }
-        if (more) put_tile(c0 + KT, buf ^ 1, idx + 1);
+        if (more) put_tile(c0 + KT, buf ^ 1);
         __syncthreads();
     }
+
+    // ---- V's non-finite values, left out of the tiles, for the rows that see them ----
+    if (bad_v)
+        for (int j = g_lo; j < min(g_end, L); j++) {
+            if (!partial(j / KT * KT)) continue;
+            const T *vr = vb + (int64_t) j * p.v_stride;
+            const bool sees = j >= lo && j < end;
+#pragma unroll
+            for (int m = 0; m < NO; m++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
+                    const float v = sees && d < p.Dv ? (float) vr[d] : 0.f;
+                    o[m][r] += (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.f;
+                }
+        }
 
     // ---- rows out ----
     l += __shfl_xor(l, 32);
