@@ -308,8 +308,8 @@ pa_prompt_kernel(PromptParams p) {
     const T *kb = (const T *) p.k + q0 * p.k_stride + (int64_t) hk * p.D;
     const T *vb = (const T *) p.v + q0 * p.v_stride + (int64_t) hk * p.Dv;
     const int pr0 = tid / CPR;   // a thread's pieces: rows pr0 + x * (threads / CPR), at one place of the row
-    auto piece_row = [&](int x) { return pr0 + x * (kPromptThreads / CPR); };
-    auto piece_dim = [&](int x, int D) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
+    auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (kPromptThreads / CPR); };
+    auto piece_dim = [&](int x, int D) __attribute__((always_inline)) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k[0]), lv0 = lds_addr(lds_v[0]);
     Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
     // 16-bit rows: byte offsets of a thread's pieces from the tile's first row
@@ -322,35 +322,35 @@ pa_prompt_kernel(PromptParams p) {
         }
     }
     const uint32_t lkw = __builtin_amdgcn_readfirstlane(lk0 + wave * 1024), lvw = __builtin_amdgcn_readfirstlane(lv0 + wave * 1024);
-    auto load_tile = [&](int c0, int buf) {
-        if constexpr (DMA) {
-            const T *kt = kb + c0 * p.k_stride, *vt = vb + c0 * p.v_stride;
-            const uint32_t ka = lkw + buf * SH::BUF, va = lvw + buf * SH::BUF;
-            if (c0 + KT <= L) {
+    // K rows ck .. of a tile into buffer bk, V rows cv .. into bv (none from g_end on)
+    auto load_rows = [&](const T *base, int64_t stride, const uint32_t (&vo)[SH::PPT], uint32_t lds, int D, int c0) __attribute__((always_inline)) {
+        const T *from = base + c0 * stride;
+        if (c0 + KT <= L) {
 #pragma unroll
-                for (int x = 0; x < SH::PPT; x++) {
-                    lds_load16_at(kt, kvo[x], ka, x * kPromptThreads * 16);
-                    lds_load16_at(vt, vvo[x], va, x * kPromptThreads * 16);
-                }
-            } else {
-#pragma unroll
-                for (int x = 0; x < SH::PPT; x++) {
-                    const uint32_t r = min(piece_row(x), L - 1 - c0);
-                    lds_load16_at(kt, (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2, ka, x * kPromptThreads * 16);
-                    lds_load16_at(vt, (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2, va, x * kPromptThreads * 16);
-                }
-            }
+            for (int x = 0; x < SH::PPT; x++) lds_load16_at(from, vo[x], lds, x * kPromptThreads * 16);
         } else {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
-                const int64_t j = min(c0 + piece_row(x), L - 1);
-                ks[x] = load_piece<TY, VEC, false>(kb + j * p.k_stride, piece_dim(x, p.D), p.D);
-                vs[x] = load_piece<TY, VEC, false>(vb + j * p.v_stride, piece_dim(x, p.Dv), p.Dv);
+                const uint32_t r = min(piece_row(x), L - 1 - c0);
+                lds_load16_at(from, (r * (uint32_t) stride + piece_dim(x, D)) * 2, lds, x * kPromptThreads * 16);
+            }
+        }
+    };
+    auto load_tile = [&](int ck, int bk, int cv, int bv) __attribute__((always_inline)) {
+        if constexpr (DMA) {
+            if (ck < g_end) load_rows(kb, p.k_stride, kvo, lkw + bk * SH::BUF, p.D, ck);
+            if (cv < g_end) load_rows(vb, p.v_stride, vvo, lvw + bv * SH::BUF, p.Dv, cv);
+        } else {
+#pragma unroll
+            for (int x = 0; x < SH::PPT; x++) {
+                const int64_t jk = min(ck + piece_row(x), L - 1), jv = min(cv + piece_row(x), L - 1);
+                if (ck < g_end) ks[x] = load_piece<TY, VEC, false>(kb + jk * p.k_stride, piece_dim(x, p.D), p.D);
+                if (cv < g_end) vs[x] = load_piece<TY, VEC, false>(vb + jv * p.v_stride, piece_dim(x, p.Dv), p.Dv);
             }
         }
     };
     // F32: the scale of a row's pieces, which are in CPR neighbouring lanes
-    auto row_scale = [&](const Piece8<TY> &x, float *up) {
+    auto row_scale = [&](const Piece8<TY> &x, float *up) __attribute__((always_inline)) {
         float m = 0.f;
         if constexpr (F32) {
 #pragma unroll
@@ -362,7 +362,7 @@ pa_prompt_kernel(PromptParams p) {
         if (tid % CPR == 0) *up = pow2(ex - 15);
         return pow2(15 - ex);
     };
-    auto put_piece = [&](const Piece8<TY> &x, char *at, float up) {
+    auto put_piece = [&](const Piece8<TY> &x, char *at, float up) __attribute__((always_inline)) {
         if constexpr (F32) {
             f16x8 hi, lw;
 #pragma unroll
@@ -379,19 +379,24 @@ pa_prompt_kernel(PromptParams p) {
         }
     };
     // (workgroup-uniform) some row of the workgroup does not see all of the tile
-    auto partial = [&](int c0) { return c0 < g_lo_all || c0 + KT > g_end_all; };
-    auto put_tile = [&](int c0, int buf) {
+    auto partial = [&](int64_t c0) __attribute__((always_inline)) { return c0 < g_lo_all || c0 + KT > g_end_all; };
+    auto put_tile = [&](int ck, int bk, int cv, int bv) __attribute__((always_inline)) {
         if constexpr (!DMA) {
             bool bad = false;
+            const bool part = partial(cv);
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
                 const int at = (tid + x * kPromptThreads) * 16, r = piece_row(x);
                 float up = 1.f;
-                if constexpr (F32) up = row_scale(ks[x], &k_up[buf][r]);
-                put_piece(ks[x], lds_k[buf] + at, up);
-                if (partial(c0)) bad |= finite_piece<TY>(vs[x]);
-                if constexpr (F32) up = row_scale(vs[x], &v_up[buf][r]);
-                put_piece(vs[x], lds_v[buf] + at, up);
+                if (ck < g_end) {
+                    if constexpr (F32) up = row_scale(ks[x], &k_up[bk][r]);
+                    put_piece(ks[x], lds_k[bk] + at, up);
+                }
+                if (cv < g_end) {
+                    if (part) bad |= finite_piece<TY>(vs[x]);
+                    if constexpr (F32) up = row_scale(vs[x], &v_up[bv][r]);
+                    put_piece(vs[x], lds_v[bv] + at, up);
+                }
             }
             if (bad) bad_v = 1;
         } else {
@@ -399,10 +404,11 @@ pa_prompt_kernel(PromptParams p) {
         }
     };
 
-    // the first tile is on its way while Q is loaded
+    // the first tile (and K of the second) is on its way while Q is loaded
     if (tid == 0) bad_v = 0;
     if constexpr (!DMA) __syncthreads();
-    if (g_lo < g_end) load_tile(g_lo, 0);
+    load_tile(g_lo, 0, g_lo, 0);
+    if constexpr (DMA) load_tile(g_lo + KT, 1, INT32_MAX, 0);
 
     // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
     u32x4 qr[NP][KS];
@@ -476,12 +482,55 @@ pa_prompt_kernel(PromptParams p) {
         for (int m = 0; m < NO; m++)
             voff[e][m] = lv0 + (vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
 
-    if (g_lo < g_end) put_tile(g_lo, 0);
-    __syncthreads();
-    int buf = 0;
-    for (int c0 = g_lo; c0 < g_end; c0 += KT, buf ^= 1) {
-        const bool more = c0 + KT < g_end;
-        if (more) load_tile(c0 + KT, buf ^ 1);
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    // The tile loop.  K is a tile ahead of V: while the weights of tile i are computed and its V multiplied, the matrix
+    // cores also take the scores of tile i + 1 into the other score registers, so that vector and matrix work of one
+    // wave overlap.  F32 has no registers for that, and takes tile i's scores at its start (AHEAD = 0).
+    constexpr int AHEAD = F32 ? 0 : 1;
+    constexpr int NQ = KS * NH;   // products of a tile's scores, and of its V (triples of them, F32)
+    static_assert(NQ == NO * (NS / 8), "as many products with K as with V");
+    u32x4 kr[3][NP], vr[3][NP];   // operands, read two products ahead
+    auto read_k = [&](int q, int buf) __attribute__((always_inline)) {
+        const int k = q / NH, hh = q % NH;
+#pragma unroll
+        for (int e = 0; e < NP; e++)
+            kr[q % 3][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE + hh * 32 * SH::STRIDE);
+    };
+    auto mul_k = [&](int q, int buf, f32x16 (&sc)[NH]) __attribute__((always_inline)) {
+        const int k = q / NH, hh = q % NH;
+        if (q + 2 < NQ) read_k(q + 2, buf);
+        if (k == 0)
+#pragma unroll
+            for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
+        sc[hh] = prompt_mfma<TY>(kr[q % 3][0], qr[0][k], sc[hh]);
+        if constexpr (F32) {
+            sc[hh] = prompt_mfma<TY>(kr[q % 3][NP - 1], qr[0][k], sc[hh]);
+            sc[hh] = prompt_mfma<TY>(kr[q % 3][0], qr[NP - 1][k], sc[hh]);
+        }
+    };
+    auto scores = [&](int buf, f32x16 (&sc)[NH]) __attribute__((always_inline)) {
+        read_k(0, buf);
+        read_k(1, buf);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < NQ; q++) {
+            mul_k(q, buf, sc);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto read_v = [&](int q, int buf) __attribute__((always_inline)) {
+        const int st = q / NO, m = q % NO;
+#pragma unroll
+        for (int e = 0; e < NP; e++) {
+            const uint32_t off = buf * SH::BUF + e * SH::PLANE + 16 * st * SH::STRIDE;
+            vr[q % 3][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
+        }
+    };
+    // Tile c0, whose V is in buffer `buf` and whose scores are sc; with AHEAD, the next tile's scores into nx.
+    auto tile = [&](int c0, auto buf_, f32x16 (&sc)[NH], f32x16 (&nx)[NH]) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_)::value;
+        const int k_at = c0 + (AHEAD + 1) * KT, v_at = c0 + KT;   // what is loaded while this tile is computed
+        load_tile(k_at, buf ^ 1 ^ AHEAD, v_at, buf ^ 1);
         if (DMA && partial(c0)) {
             bool bad = false;
 #pragma unroll
@@ -497,41 +546,7 @@ pa_prompt_kernel(PromptParams p) {
             __syncthreads();
         }
         if (c0 < w_end && c0 + KT > w_lo) {   // wave-uniform: some row sees some of the tile
-            typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-            // ---- scores ----
-            f32x16 sc[NH];
-#pragma unroll
-            for (int hh = 0; hh < NH; hh++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
-            const uint32_t bo = buf * SH::BUF;
-            // Operands are read two products' worth ahead; the scheduling barriers keep the compiler from pulling
-            // each read down to its product, where the wave would wait for it.
-            u32x4 kr[3][NH][NP];
-            auto read_k = [&](int k) {
-                const uint32_t at = koff[k] + bo;
-#pragma unroll
-                for (int hh = 0; hh < NH; hh++)
-#pragma unroll
-                    for (int e = 0; e < NP; e++)
-                        kr[k % 3][hh][e] = *(const lds_u32x4 *) (uintptr_t) (at + e * SH::PLANE + hh * 32 * SH::STRIDE);
-            };
-            read_k(0);
-            read_k(1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                if (k + 2 < KS) read_k(k + 2);
-#pragma unroll
-                for (int hh = 0; hh < NH; hh++) {
-                    sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][0], qr[0][k], sc[hh]);
-                    if constexpr (F32) {
-                        sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][NP - 1], qr[0][k], sc[hh]);
-                        sc[hh] = prompt_mfma<TY>(kr[k % 3][hh][0], qr[NP - 1][k], sc[hh]);
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            if constexpr (!AHEAD) scores(buf, sc);
             // ---- softmax ----
             float x[NS];
             float cx = cs;   // x times cx is the score in log2 units
@@ -555,6 +570,12 @@ pa_prompt_kernel(PromptParams p) {
                     const int key = (j / 16) * 32 + 8 * (j % 16 / 4) + j % 4;
                     x[j] = key >= a && key < b ? x[j] : -INFINITY;
                 }
+            }
+            if constexpr (AHEAD) {
+                read_k(0, buf ^ 1);
+                read_k(1, buf ^ 1);
+#pragma unroll
+                for (int q = 0; q < NQ / 4; q++) mul_k(q, buf ^ 1, nx);
             }
             float mx = x[0];
 #pragma unroll
@@ -613,46 +634,57 @@ pa_prompt_kernel(PromptParams p) {
             }
             // ---- O^T += V^T P^T, the next 16 tokens' probabilities beside the products of 16 ----
             // (the sum is of the rounded probabilities, as the products are)
-            auto weigh = [&](int st, int e) {   // pair e of the 16 tokens st
+            auto weigh = [&](int st, int e) __attribute__((always_inline)) {   // pair e of the 16 tokens st
                 x[8 * st + 2 * e] = __builtin_amdgcn_exp2f(fmaf(x[8 * st + 2 * e], cx, -ref));
                 x[8 * st + 2 * e + 1] = __builtin_amdgcn_exp2f(fmaf(x[8 * st + 2 * e + 1], cx, -ref));
                 pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
                 l = sum2<TY>(pr[0][st][e], l);
             };
-            constexpr int NQ = NO * (NS / 8);   // products (triples of them, F32)
-            u32x4 vr[3][NP];
-            auto read_v = [&](int q) {
-                const int st = q / NO, m = q % NO;
-#pragma unroll
-                for (int e = 0; e < NP; e++) {
-                    const uint32_t off = bo + e * SH::PLANE + 16 * st * SH::STRIDE;
-                    vr[q % 3][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
-                }
-            };
-            read_v(0);
-            read_v(1);
+            read_v(0, buf);
+            read_v(1, buf);
             if constexpr (!F32) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) weigh(0, e);
+#pragma unroll
+                for (int q = NQ / 4; q < NQ / 2; q++) mul_k(q, buf ^ 1, nx);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int q = 0; q < NQ; q++) {
                 const int st = q / NO, m = q % NO;
-                if (q + 2 < NQ) read_v(q + 2);
+                if (q + 2 < NQ) read_v(q + 2, buf);
                 o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[0][st], o[m]);
                 if constexpr (F32) {
                     o[m] = prompt_mfma<TY>(vr[q % 3][NP - 1], pr[0][st], o[m]);
                     o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[NP - 1][st], o[m]);
-                } else if (st + 1 < NS / 8) {
+                } else {
+                    if (q % 2 == 0) mul_k(NQ / 2 + q / 2, buf ^ 1, nx);
+                    if (st + 1 < NS / 8) {
 #pragma unroll
-                    for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
+                        for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
+                    }
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+        } else if constexpr (AHEAD) {
+            scores(buf ^ 1, nx);
         }
-        if (more) put_tile(c0 + KT, buf ^ 1);
+        put_tile(k_at, buf ^ 1 ^ AHEAD, v_at, buf ^ 1);
         __syncthreads();
+    };
+    f32x16 s0[NH], s1[NH];
+    put_tile(g_lo, 0, g_lo, 0);
+    __syncthreads();
+    if constexpr (AHEAD) {
+        if constexpr (!DMA) load_tile(g_lo + KT, 1, INT32_MAX, 0);
+        scores(0, s0);
+        if constexpr (!DMA) put_tile(g_lo + KT, 1, INT32_MAX, 0);
+        __syncthreads();
+    }
+    for (int c0 = g_lo; c0 < g_end; c0 += 2 * KT) {
+        tile(c0, std::integral_constant<int, 0>(), s0, s1);
+        if (c0 + KT >= g_end) break;
+        tile(c0 + KT, std::integral_constant<int, 1>(), s1, s0);
     }
 
     // ---- V's non-finite values, left out of the tiles, for the rows that see them ----
