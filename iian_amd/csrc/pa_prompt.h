@@ -4,9 +4,11 @@
 //
 // A workgroup of 4 waves owns 128 rows r = i*gqa + g (token i, head g of the
 // group) of one (prompt, kv head), 32 per wave, and walks the tokens that any of
-// them sees in tiles of KT, staged in LDS (two buffers, one barrier per tile: the
-// next tile's rows are requested before the tile is computed and written behind
-// it).  One pass with a running maximum and sum per row:
+// them sees in tiles of 32, staged in LDS two tiles ahead (one ahead through
+// registers), one barrier per tile.  Calls with fewer workgroups than that fills
+// the chip with split the tokens instead (KW > 1): KW waves share 32 rows, each
+// takes every KW-th tile, and their results are joined in LDS at the end.  One
+// pass with a running maximum and sum per row:
 //
 //   S^T = K Q^T     v_mfma_f32_32x32x16: K rows are the A operand as they lie in
 //                   LDS, Q^T stays in registers.  Lane l then holds, of row l%32,
@@ -43,7 +45,7 @@ namespace iian_pa {
 
 constexpr int kPromptWaves = 4;
 constexpr int kPromptThreads = kPromptWaves * 64;
-constexpr int kPromptRows = kPromptWaves * 32;   // rows per workgroup
+constexpr int kPromptSplitBlocks = 256;   // blocks of 128 rows up to which waves share rows
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -63,24 +65,31 @@ struct PromptType<0> {
     typedef float T;
 };
 
-// TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32.
+// TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32; VEC: rows of
+// whole aligned 16-byte pieces; KW: waves that share their rows.
 //
 // LDS tiles.  Rows are unpadded, so that tiles of 16-bit rows can be loaded
 // straight into LDS (16 consecutive bytes per lane), and the 16-byte pieces of
 // row r are permuted by an exclusive or with swz(r) instead: 16 rows read at one
 // piece, as QK^T does, and the 4 rows x 64 bytes of a transpose read each fill
 // the 64 banks.
-template <int TY, int DK, int DV>
+template <int TY, int DK, int DV, bool VEC, int KW>
 struct PromptShape {
-    static constexpr int NP = TY == 0 ? 2 : 1;                 // 16-bit terms per value
-    static constexpr int KT = TY == 0 || DK > 128 ? 32 : 64;   // tokens per tile
-    static constexpr int NH = KT / 32, KS = DK / 16, NO = DV / 32;
+    static constexpr int NP = TY == 0 ? 2 : 1;             // 16-bit terms per value
+    static constexpr bool DMA = VEC && TY != 0;            // tiles go straight into LDS
+    static constexpr int KT = 32, TT = KT * KW;            // tokens per wave and tile, and per workgroup's
+    static constexpr int ROWS = 32 * (kPromptWaves / KW);  // rows per workgroup
+    static constexpr int KS = DK / 16, NO = DV / 32, NS = 16;
     static constexpr int CPR = DK <= 64 ? 8 : DK <= 128 ? 16 : 32;   // 16-byte pieces per row
     static_assert((DV <= 64 ? 8 : DV <= 128 ? 16 : 32) == CPR, "K and V rows of one pitch");
     static constexpr int STRIDE = CPR * 16;
-    static constexpr int PLANE = KT * STRIDE, BUF = NP * PLANE;
-    static constexpr int PPT = KT * CPR / kPromptThreads;      // pieces per thread and tile
-    static_assert(PPT * kPromptThreads == KT * CPR, "pieces divide evenly");
+    static constexpr int PLANE = TT * STRIDE, BUF = NP * PLANE;
+    // three buffers (loads two tiles ahead) where three workgroups of them fit a CU's 160 KB of LDS
+    static constexpr int NB = DMA && BUF * 6 <= 49152 ? 3 : 2;
+    static constexpr int PPT = TT * CPR / kPromptThreads;  // pieces per thread and tile
+    static_assert(PPT * kPromptThreads == TT * CPR, "pieces divide evenly");
+    // waves per SIMD asked of the register allocator
+    static constexpr int WAVES = DK > 128 ? 1 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
     __device__ static __forceinline__ int swz(int r) {
         return CPR == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -212,56 +221,122 @@ __device__ __forceinline__ bool finite_piece(Piece8<TY> &x) {
     return bad;
 }
 
-// Row block b of the launch: the prompts' blocks in order, each prompt's last
-// (which sees the most tokens) first.  Wave-uniform; false past the last.
-__device__ __forceinline__ bool find_block(const PromptParams &p, int b, int &s, int &rb, int &q0, int &L) {
-    const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int s0 = 0; s0 < p.S; s0 += 64) {
-        const int si = s0 + lane;
-        int a = 0, len = 0, n = 0;
-        if (si < p.S) {
-            a = min(max(p.qsl[si], 0), p.T);
-            len = min(max(p.qsl[si + 1], a), p.T) - a;
-            n = (int) (((int64_t) min(len, p.max_q) * p.gqa + kPromptRows - 1) / kPromptRows);
-        }
-        const int sum = wave_incl_scan(n);
-        const int total = __builtin_amdgcn_readlane(sum, 63);
-        if (b < base + total) {
-            const uint64_t m = __ballot(base + sum > b);
-            const int at = __builtin_ctzll(m);
-            s = s0 + at;
-            q0 = __builtin_amdgcn_readlane(a, at);
-            L = __builtin_amdgcn_readlane(len, at);
-            rb = base + __builtin_amdgcn_readlane(sum, at) - 1 - b;   // the last block first
-            return true;
-        }
-        base += total;
-    }
-    return false;
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ int lane_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast 15 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast 31 into rows 2 and 3
+    return v;
 }
 
-template <int TY, int DK, int DV, bool VEC>
-__global__ __launch_bounds__(kPromptThreads) __attribute__((amdgpu_waves_per_eu(DK <= 128 ? 2 : 1))) void
-pa_prompt_kernel(PromptParams p) {
-    using SH = PromptShape<TY, DK, DV>;
+struct PromptBlock {
+    int s, rb, q0, L;   // prompt, row block, first token, tokens
+};
+
+// Row block b of the launch, in an order that starts the longest work first:
+// with up to 64 prompts, causal ones by row block, the last of any prompt first
+// (a row block's work grows with its place in the prompt), others by the
+// prompt's length.  More prompts: in order, each prompt's last block first.
+// Wave-uniform; false past the last block.
+template <int ROWS>
+__device__ __forceinline__ bool find_block(const PromptParams &p, int b, PromptBlock &out) {
+    const int lane = threadIdx.x & 63;
+    auto prompt = [&](int s, int &a, int &len) {
+        a = min(max(p.qsl[s], 0), p.T);
+        len = min(max(p.qsl[s + 1], a), p.T) - a;
+        return (int) (((int64_t) min(len, p.max_q) * p.gqa + ROWS - 1) / ROWS);
+    };
+    int a = 0, len = 0, n = 0, s0 = 0;
+    if (p.S <= 64) {
+        if (lane < p.S) n = prompt(lane, a, len);
+        if (p.S > 1) {
+            int at, rb;
+            if (p.causal || p.row_end) {
+                // the largest row block index r with more than b blocks at r or above
+                int lo = 0, above = 0, hi = INT32_MAX;   // sum over prompts of max(0, n - lo) > b; at hi it is not
+                const int all = __builtin_amdgcn_readlane(lane_scan(n), 63);
+                if (b >= all) return false;
+                for (hi = all; hi - lo > 1;) {
+                    const int m = (lo + hi) >> 1, c = __builtin_amdgcn_readlane(lane_scan(max(0, n - m)), 63);
+                    if (c > b) lo = m;
+                    else hi = m, above = c;
+                }
+                uint64_t m = __ballot(n > lo);
+                for (int k = b - above; k > 0; k--) m &= m - 1;
+                at = __builtin_ctzll(m);
+                rb = lo;
+            } else {
+                int before = 0;   // blocks of longer prompts, and of earlier ones as long
+                for (int j = 0; j < p.S; j++) {
+                    const int nj = __builtin_amdgcn_readlane(n, j);
+                    before += nj > n || (nj == n && j < lane) ? nj : 0;
+                }
+                const uint64_t m = __ballot(b >= before && b < before + n);
+                if (!m) return false;
+                at = __builtin_ctzll(m);
+                rb = b - __builtin_amdgcn_readlane(before, at);
+            }
+            out = {at, rb, __builtin_amdgcn_readlane(a, at), __builtin_amdgcn_readlane(len, at)};
+            return true;
+        }
+    } else {
+        // the lane's share of the prompts, then the prompts of the share that holds b
+        const int per = (p.S + 63) / 64;
+        int sum = 0;
+        for (int s = lane * per; s < min(p.S, (lane + 1) * per); s++) sum += prompt(s, a, len);
+        const int scan = lane_scan(sum);
+        const uint64_t m = __ballot(scan > b);
+        if (!m) return false;
+        const int at = __builtin_ctzll(m);
+        b -= __builtin_amdgcn_readlane(scan, at) - __builtin_amdgcn_readlane(sum, at);
+        s0 = at * per;
+        n = 0;
+        if (s0 + lane < p.S) n = prompt(s0 + lane, a, len);
+    }
+    for (;;) {
+        const int scan = lane_scan(n), all = __builtin_amdgcn_readlane(scan, 63);
+        if (b < all) {
+            const int at = __builtin_ctzll(__ballot(scan > b));
+            out = {s0 + at, __builtin_amdgcn_readlane(scan, at) - 1 - b, __builtin_amdgcn_readlane(a, at),
+                   __builtin_amdgcn_readlane(len, at)};
+            return true;
+        }
+        b -= all;
+        s0 += 64;
+        if (s0 >= p.S) return false;
+        n = 0;
+        if (s0 + lane < p.S) n = prompt(s0 + lane, a, len);
+    }
+}
+
+template <int TY, int DK, int DV, bool VEC, int KW>
+__global__ __launch_bounds__(kPromptThreads)
+    __attribute__((amdgpu_waves_per_eu(PromptShape<TY, DK, DV, VEC, KW>::WAVES))) void pa_prompt_kernel(PromptParams p) {
+    using SH = PromptShape<TY, DK, DV, VEC, KW>;
     using T = typename PromptType<TY>::T;
-    constexpr bool F32 = TY == 0, DMA = VEC && !F32;   // 16-bit tiles go straight into LDS
-    constexpr int NP = SH::NP, KT = SH::KT, NH = SH::NH, KS = SH::KS, NO = SH::NO, NS = 16 * NH, CPR = SH::CPR;
-    __shared__ __attribute__((aligned(16))) char lds_k[2][SH::BUF];
-    __shared__ __attribute__((aligned(16))) char lds_v[2][SH::BUF];
-    __shared__ __attribute__((aligned(16))) float k_up[2][F32 ? KT : 1];   // F32: 2^(e - 15) of each K row
-    __shared__ __attribute__((aligned(16))) float v_up[2][F32 ? KT : 1];   // and of each V row
+    constexpr bool F32 = TY == 0, DMA = SH::DMA;
+    constexpr int NP = SH::NP, KT = SH::KT, TT = SH::TT, NB = SH::NB, KS = SH::KS, NO = SH::NO, NS = SH::NS, CPR = SH::CPR;
+    constexpr int ROWS = SH::ROWS;
+    // K and V tiles; in the end the waves' results that are joined
+    constexpr int JOIN = KW > 1 ? kPromptWaves * (NO * 16 + 2) * 64 * 4 : 0;
+    __shared__ __attribute__((aligned(16))) char lds[std::max(2 * NB * SH::BUF, JOIN)];
+    char *const lds_k = lds, *const lds_v = lds + NB * SH::BUF;
+    __shared__ __attribute__((aligned(16))) float k_up[NB][F32 ? TT : 1];   // F32: 2^(e - 15) of each K row
+    __shared__ __attribute__((aligned(16))) float v_up[NB][F32 ? TT : 1];   // and of each V row
     __shared__ int bad_v;   // some tile that is not seen whole had non-finite values of V (left out of it)
     __shared__ int wave_end[2][kPromptWaves];
 
     const int hk = blockIdx.x % p.Hkv;
-    int s, rb, q0, L;
-    if (!find_block(p, blockIdx.x / p.Hkv, s, rb, q0, L)) return;
+    PromptBlock blk;
+    if (!find_block<ROWS>(p, blockIdx.x / p.Hkv, blk)) return;
+    const int q0 = blk.q0, L = blk.L;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
-    if (rb == 0 && hk == 0 && tid == 0 && L > p.max_q && p.err) atomicOr(p.err, 4);
+    if (blk.rb == 0 && hk == 0 && tid == 0 && L > p.max_q && p.err) atomicOr(p.err, 4);
     const int rows = min(L, p.max_q) * p.gqa;   // (the host holds tokens times heads below 2^31)
-    const int wg0 = rb * kPromptRows, row0 = wg0 + 32 * wave;
+    const int wg0 = blk.rb * ROWS, row0 = wg0 + 32 * (wave / KW), kg = wave % KW;
 
     // ---- the wave's rows: token i of the lane's row, and the tokens it sees, [lo, end) ----
     const int row = row0 + n;
@@ -274,7 +349,7 @@ pa_prompt_kernel(PromptParams p) {
     // of the wave: the tokens that all of its rows see, [w_lo_all, w_end_all), and that any sees, [w_lo, w_end)
     const int last = min(row0 + 31, rows - 1), i_first = row0 / p.gqa, i_last = last / p.gqa;
     // of the workgroup: its tiles start in [g_lo, g_end), and all of its rows see [g_lo_all, g_end_all)
-    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + kPromptRows, rows) - 1) / p.gqa;
+    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + ROWS, rows) - 1) / p.gqa;
     int w_end, w_end_all, g_end, g_end_all;
     if (p.row_end) {
         int mx = end, mn = live ? end : INT32_MAX;
@@ -300,7 +375,7 @@ pa_prompt_kernel(PromptParams p) {
     }
     const int w_lo = p.n_swa > 0 ? max(0, i_first - p.n_swa + 1) : 0;
     const int w_lo_all = p.n_swa > 0 ? max(0, i_last - p.n_swa + 1) : 0;
-    const int g_lo = (p.n_swa > 0 ? max(0, g_first - p.n_swa + 1) : 0) / KT * KT;
+    const int g_lo = (p.n_swa > 0 ? max(0, g_first - p.n_swa + 1) : 0) / TT * TT;
     const int g_lo_all = p.n_swa > 0 ? max(0, g_last - p.n_swa + 1) : 0;
 
     // ---- staging: piece (row r, 8 dims) of a tile per thread and step; rows past the prompt's end
@@ -310,7 +385,7 @@ pa_prompt_kernel(PromptParams p) {
     const int pr0 = tid / CPR;   // a thread's pieces: rows pr0 + x * (threads / CPR), at one place of the row
     auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (kPromptThreads / CPR); };
     auto piece_dim = [&](int x, int D) __attribute__((always_inline)) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
-    const uint32_t lk0 = lds_addr(lds_k[0]), lv0 = lds_addr(lds_v[0]);
+    const uint32_t lk0 = lds_addr(lds_k), lv0 = lds_addr(lds_v);
     Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
     // 16-bit rows: byte offsets of a thread's pieces from the tile's first row
     uint32_t kvo[SH::PPT], vvo[SH::PPT];
@@ -322,10 +397,10 @@ pa_prompt_kernel(PromptParams p) {
         }
     }
     const uint32_t lkw = __builtin_amdgcn_readfirstlane(lk0 + wave * 1024), lvw = __builtin_amdgcn_readfirstlane(lv0 + wave * 1024);
-    // K rows ck .. of a tile into buffer bk, V rows cv .. into bv (none from g_end on)
+    // Rows c0 .. of a tile into LDS, or registers; nothing from g_end on.
     auto load_rows = [&](const T *base, int64_t stride, const uint32_t (&vo)[SH::PPT], uint32_t lds, int D, int c0) __attribute__((always_inline)) {
         const T *from = base + c0 * stride;
-        if (c0 + KT <= L) {
+        if (c0 + TT <= L) {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) lds_load16_at(from, vo[x], lds, x * kPromptThreads * 16);
         } else {
@@ -336,16 +411,17 @@ pa_prompt_kernel(PromptParams p) {
             }
         }
     };
-    auto load_tile = [&](int ck, int bk, int cv, int bv) __attribute__((always_inline)) {
+    auto load_tile = [&](int c0, int buf) __attribute__((always_inline)) {
+        if (c0 >= g_end) return;
         if constexpr (DMA) {
-            if (ck < g_end) load_rows(kb, p.k_stride, kvo, lkw + bk * SH::BUF, p.D, ck);
-            if (cv < g_end) load_rows(vb, p.v_stride, vvo, lvw + bv * SH::BUF, p.Dv, cv);
+            load_rows(kb, p.k_stride, kvo, lkw + buf * SH::BUF, p.D, c0);
+            load_rows(vb, p.v_stride, vvo, lvw + buf * SH::BUF, p.Dv, c0);
         } else {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
-                const int64_t jk = min(ck + piece_row(x), L - 1), jv = min(cv + piece_row(x), L - 1);
-                if (ck < g_end) ks[x] = load_piece<TY, VEC, false>(kb + jk * p.k_stride, piece_dim(x, p.D), p.D);
-                if (cv < g_end) vs[x] = load_piece<TY, VEC, false>(vb + jv * p.v_stride, piece_dim(x, p.Dv), p.Dv);
+                const int64_t j = min(c0 + piece_row(x), L - 1);
+                ks[x] = load_piece<TY, VEC, false>(kb + j * p.k_stride, piece_dim(x, p.D), p.D);
+                vs[x] = load_piece<TY, VEC, false>(vb + j * p.v_stride, piece_dim(x, p.Dv), p.Dv);
             }
         }
     };
@@ -379,36 +455,35 @@ pa_prompt_kernel(PromptParams p) {
         }
     };
     // (workgroup-uniform) some row of the workgroup does not see all of the tile
-    auto partial = [&](int64_t c0) __attribute__((always_inline)) { return c0 < g_lo_all || c0 + KT > g_end_all; };
-    auto put_tile = [&](int ck, int bk, int cv, int bv) __attribute__((always_inline)) {
+    auto partial = [&](int c0) __attribute__((always_inline)) { return c0 < g_lo_all || c0 + TT > g_end_all; };
+    // Loaded rows into LDS; or the wait for tile c0, behind which `newer` tiles may still be on their way.
+    auto put_tile = [&](int c0, int buf, bool newer) __attribute__((always_inline)) {
         if constexpr (!DMA) {
+            if (c0 >= g_end) return;
             bool bad = false;
-            const bool part = partial(cv);
+            const bool part = partial(c0);
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
-                const int at = (tid + x * kPromptThreads) * 16, r = piece_row(x);
+                const int at = buf * SH::BUF + (tid + x * kPromptThreads) * 16, r = piece_row(x);
                 float up = 1.f;
-                if (ck < g_end) {
-                    if constexpr (F32) up = row_scale(ks[x], &k_up[bk][r]);
-                    put_piece(ks[x], lds_k[bk] + at, up);
-                }
-                if (cv < g_end) {
-                    if (part) bad |= finite_piece<TY>(vs[x]);
-                    if constexpr (F32) up = row_scale(vs[x], &v_up[bv][r]);
-                    put_piece(vs[x], lds_v[bv] + at, up);
-                }
+                if constexpr (F32) up = row_scale(ks[x], &k_up[buf][r]);
+                put_piece(ks[x], lds_k + at, up);
+                if (part) bad |= finite_piece<TY>(vs[x]);
+                if constexpr (F32) up = row_scale(vs[x], &v_up[buf][r]);
+                put_piece(vs[x], lds_v + at, up);
             }
             if (bad) bad_v = 1;
         } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if (newer) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * SH::PPT) : "memory");
+            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
 
-    // the first tile (and K of the second) is on its way while Q is loaded
+    // the first tiles are on their way while Q is loaded
     if (tid == 0) bad_v = 0;
     if constexpr (!DMA) __syncthreads();
-    load_tile(g_lo, 0, g_lo, 0);
-    if constexpr (DMA) load_tile(g_lo + KT, 1, INT32_MAX, 0);
+    load_tile(g_lo, 0);
+    if constexpr (NB == 3) load_tile(g_lo + TT, 1);
 
     // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
     u32x4 qr[NP][KS];
@@ -475,48 +550,23 @@ pa_prompt_kernel(PromptParams p) {
     const int vrow = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     uint32_t koff[KS], voff[2][NO];
 #pragma unroll
-    for (int k = 0; k < KS; k++) koff[k] = lk0 + n * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n));
+    for (int k = 0; k < KS; k++) koff[k] = lk0 + (KT * kg + n) * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n));
 #pragma unroll
     for (int e = 0; e < 2; e++)
 #pragma unroll
         for (int m = 0; m < NO; m++)
-            voff[e][m] = lv0 + (vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
+            voff[e][m] = lv0 + (KT * kg + vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
 
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-    // The tile loop.  K is a tile ahead of V: while the weights of tile i are computed and its V multiplied, the matrix
-    // cores also take the scores of tile i + 1 into the other score registers, so that vector and matrix work of one
-    // wave overlap.  F32 has no registers for that, and takes tile i's scores at its start (AHEAD = 0).
-    constexpr int AHEAD = F32 ? 0 : 1;
-    constexpr int NQ = KS * NH;   // products of a tile's scores, and of its V (triples of them, F32)
-    static_assert(NQ == NO * (NS / 8), "as many products with K as with V");
-    u32x4 kr[3][NP], vr[3][NP];   // operands, read two products ahead
-    auto read_k = [&](int q, int buf) __attribute__((always_inline)) {
-        const int k = q / NH, hh = q % NH;
+    // ---- the tile loop ----
+    // Operands are read two products ahead; the scheduling barriers keep the compiler from pulling each read down to its
+    // product, where the wave would wait for it.
+    constexpr int NQ = NO * (NS / 8);   // products (triples of them, F32) of a tile with V; KS with K
+    u32x4 kr[3][NP], vr[3][NP];
+    auto read_k = [&](int k, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < NP; e++)
-            kr[q % 3][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE + hh * 32 * SH::STRIDE);
-    };
-    auto mul_k = [&](int q, int buf, f32x16 (&sc)[NH]) __attribute__((always_inline)) {
-        const int k = q / NH, hh = q % NH;
-        if (q + 2 < NQ) read_k(q + 2, buf);
-        if (k == 0)
-#pragma unroll
-            for (int r = 0; r < 16; r++) sc[hh][r] = 0.f;
-        sc[hh] = prompt_mfma<TY>(kr[q % 3][0], qr[0][k], sc[hh]);
-        if constexpr (F32) {
-            sc[hh] = prompt_mfma<TY>(kr[q % 3][NP - 1], qr[0][k], sc[hh]);
-            sc[hh] = prompt_mfma<TY>(kr[q % 3][0], qr[NP - 1][k], sc[hh]);
-        }
-    };
-    auto scores = [&](int buf, f32x16 (&sc)[NH]) __attribute__((always_inline)) {
-        read_k(0, buf);
-        read_k(1, buf);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int q = 0; q < NQ; q++) {
-            mul_k(q, buf, sc);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+            kr[k % 3][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE);
     };
     auto read_v = [&](int q, int buf) __attribute__((always_inline)) {
         const int st = q / NO, m = q % NO;
@@ -526,17 +576,16 @@ pa_prompt_kernel(PromptParams p) {
             vr[q % 3][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
         }
     };
-    // Tile c0, whose V is in buffer `buf` and whose scores are sc; with AHEAD, the next tile's scores into nx.
-    auto tile = [&](int c0, auto buf_, f32x16 (&sc)[NH], f32x16 (&nx)[NH]) __attribute__((always_inline)) {
-        constexpr int buf = decltype(buf_)::value;
-        const int k_at = c0 + (AHEAD + 1) * KT, v_at = c0 + KT;   // what is loaded while this tile is computed
-        load_tile(k_at, buf ^ 1 ^ AHEAD, v_at, buf ^ 1);
+    // Tile c0 of the workgroup, in buffer buf_: the wave's part of it begins at cw.
+    auto tile = [&](int c0, auto buf_) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_)::value, ahead = (buf + NB - 1) % NB;   // ahead: the tile that is loaded meanwhile
+        load_tile(c0 + (NB - 1) * TT, ahead);
         if (DMA && partial(c0)) {
             bool bad = false;
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
                 Piece8<TY> v;
-                u32x4 *at = (u32x4 *) (lds_v[buf] + (tid + x * kPromptThreads) * 16);
+                u32x4 *at = (u32x4 *) (lds_v + buf * SH::BUF + (tid + x * kPromptThreads) * 16);
                 if constexpr (!F32) {
                     v.a = *at;
                     if (finite_piece<TY>(v)) *at = v.a, bad = true;
@@ -545,15 +594,32 @@ pa_prompt_kernel(PromptParams p) {
             if (bad) bad_v = 1;
             __syncthreads();
         }
-        if (c0 < w_end && c0 + KT > w_lo) {   // wave-uniform: some row sees some of the tile
-            if constexpr (!AHEAD) scores(buf, sc);
+        const int cw = c0 + KT * kg;
+        if (cw < w_end && cw + KT > w_lo) {   // wave-uniform: some row sees some of it
+            // ---- scores ----
+            f32x16 sc;
+#pragma unroll
+            for (int r = 0; r < 16; r++) sc[r] = 0.f;
+            read_k(0, buf);
+            read_k(1, buf);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                if (k + 2 < KS) read_k(k + 2, buf);
+                sc = prompt_mfma<TY>(kr[k % 3][0], qr[0][k], sc);
+                if constexpr (F32) {
+                    sc = prompt_mfma<TY>(kr[k % 3][NP - 1], qr[0][k], sc);
+                    sc = prompt_mfma<TY>(kr[k % 3][0], qr[NP - 1][k], sc);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             // ---- softmax ----
             float x[NS];
             float cx = cs;   // x times cx is the score in log2 units
 #pragma unroll
             for (int j = 0; j < NS; j++) {
-                x[j] = sc[j / 16][j % 16];
-                if constexpr (F32) x[j] *= k_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
+                x[j] = sc[j];
+                if constexpr (F32) x[j] *= k_up[buf][KT * kg + 8 * (j / 4) + 4 * h + j % 4];
             }
             if (p.softcap > 0.f) {
 #pragma unroll
@@ -563,19 +629,13 @@ pa_prompt_kernel(PromptParams p) {
                 }
                 cx = p.softcap * kLog2e;
             }
-            if (c0 < w_lo_all || c0 + KT > w_end_all) {   // wave-uniform
-                const int a = lo - c0 - 4 * h, b = end - c0 - 4 * h;
+            if (cw < w_lo_all || cw + KT > w_end_all) {   // wave-uniform
+                const int a = lo - cw - 4 * h, b = end - cw - 4 * h;
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
-                    const int key = (j / 16) * 32 + 8 * (j % 16 / 4) + j % 4;
+                    const int key = 8 * (j / 4) + j % 4;
                     x[j] = key >= a && key < b ? x[j] : -INFINITY;
                 }
-            }
-            if constexpr (AHEAD) {
-                read_k(0, buf ^ 1);
-                read_k(1, buf ^ 1);
-#pragma unroll
-                for (int q = 0; q < NQ / 4; q++) mul_k(q, buf ^ 1, nx);
             }
             float mx = x[0];
 #pragma unroll
@@ -603,7 +663,7 @@ pa_prompt_kernel(PromptParams p) {
                 float vf[NS], top = 0.f;
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
-                    vf[j] = v_up[buf][(j / 16) * 32 + 8 * (j % 16 / 4) + 4 * h + j % 4];
+                    vf[j] = v_up[buf][KT * kg + 8 * (j / 4) + 4 * h + j % 4];
                     top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
                 }
                 top = max_halves(top);
@@ -645,8 +705,6 @@ pa_prompt_kernel(PromptParams p) {
             if constexpr (!F32) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) weigh(0, e);
-#pragma unroll
-                for (int q = NQ / 4; q < NQ / 2; q++) mul_k(q, buf ^ 1, nx);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -657,46 +715,81 @@ pa_prompt_kernel(PromptParams p) {
                 if constexpr (F32) {
                     o[m] = prompt_mfma<TY>(vr[q % 3][NP - 1], pr[0][st], o[m]);
                     o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[NP - 1][st], o[m]);
-                } else {
-                    if (q % 2 == 0) mul_k(NQ / 2 + q / 2, buf ^ 1, nx);
-                    if (st + 1 < NS / 8) {
+                } else if (st + 1 < NS / 8) {
 #pragma unroll
-                        for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
-                    }
+                    for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        } else if constexpr (AHEAD) {
-            scores(buf ^ 1, nx);
         }
-        put_tile(k_at, buf ^ 1 ^ AHEAD, v_at, buf ^ 1);
+        put_tile(c0 + TT, (buf + 1) % NB, c0 + (NB - 1) * TT < g_end && NB == 3);
         __syncthreads();
     };
-    f32x16 s0[NH], s1[NH];
-    put_tile(g_lo, 0, g_lo, 0);
+    put_tile(g_lo, 0, NB == 3 && g_lo + TT < g_end);
     __syncthreads();
-    if constexpr (AHEAD) {
-        if constexpr (!DMA) load_tile(g_lo + KT, 1, INT32_MAX, 0);
-        scores(0, s0);
-        if constexpr (!DMA) put_tile(g_lo + KT, 1, INT32_MAX, 0);
-        __syncthreads();
+    for (int c0 = g_lo; c0 < g_end; c0 += NB * TT) {
+        tile(c0, std::integral_constant<int, 0>());
+        if (c0 + TT >= g_end) break;
+        tile(c0 + TT, std::integral_constant<int, 1>());
+        if constexpr (NB == 3) {
+            if (c0 + 2 * TT >= g_end) break;
+            tile(c0 + 2 * TT, std::integral_constant<int, 2>());
+        }
     }
-    for (int c0 = g_lo; c0 < g_end; c0 += 2 * KT) {
-        tile(c0, std::integral_constant<int, 0>(), s0, s1);
-        if (c0 + KT >= g_end) break;
-        tile(c0 + KT, std::integral_constant<int, 1>(), s1, s0);
+
+    l += __shfl_xor(l, 32);
+    // ---- KW > 1: the waves' results joined; each wave then has every KW-th 32 dims of its rows ----
+    if constexpr (KW > 1) {
+        float *const mine = (float *) lds + (wave * (NO * 16 + 2)) * 64 + lane;
+        if constexpr (F32) {   // in units of their own rows' V
+#pragma unroll
+            for (int m = 0; m < NO; m++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[m][r] *= v_ref;
+        }
+        // (the loop ended with a barrier: the tiles are read)
+#pragma unroll
+        for (int m = 0; m < NO; m++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mine[(m * 16 + r) * 64] = o[m][r];
+        mine[NO * 16 * 64] = m_ref;
+        mine[(NO * 16 + 1) * 64] = l;
+        __syncthreads();
+        const float *const first = (const float *) lds + (wave / KW * KW * (NO * 16 + 2)) * 64 + lane;
+        float f[KW], top = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; w++) top = fmaxf(top, first[(w * (NO * 16 + 2) + NO * 16) * 64]);
+#pragma unroll
+        for (int w = 0; w < KW; w++) {
+            f[w] = __builtin_amdgcn_exp2f(first[(w * (NO * 16 + 2) + NO * 16) * 64] - top);
+            l += f[w] * first[(w * (NO * 16 + 2) + NO * 16 + 1) * 64];
+        }
+#pragma unroll
+        for (int m = 0; m < NO; m++) {
+            if (m % KW != kg) continue;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float sum = 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; w++) sum += f[w] * first[(w * (NO * 16 + 2) + m * 16 + r) * 64];
+                o[m][r] = sum;
+            }
+        }
     }
 
     // ---- V's non-finite values, left out of the tiles, for the rows that see them ----
+    // (each value by the one wave that stores its place)
     if (bad_v)
         for (int j = g_lo; j < min(g_end, L); j++) {
-            if (!partial(j / KT * KT)) continue;
+            if (!partial(j / TT * TT)) continue;
             const T *vr = vb + (int64_t) j * p.v_stride;
             const bool sees = j >= lo && j < end;
 #pragma unroll
             for (int m = 0; m < NO; m++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
+                    if (KW > 1 && m % KW != kg) continue;
                     const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
                     const float v = sees && d < p.Dv ? (float) vr[d] : 0.f;
                     o[m][r] += (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.f;
@@ -704,15 +797,15 @@ pa_prompt_kernel(PromptParams p) {
         }
 
     // ---- rows out ----
-    l += __shfl_xor(l, 32);
     float inv = l == 0.f ? 0.f : 1.f / l;
     if (!live) return;
-    if constexpr (F32) inv *= v_ref;   // (an empty row: 0 * 2^-126)
+    if constexpr (F32 && KW == 1) inv *= v_ref;   // (an empty row: 0 * 2^-126)
     T *out = (T *) p.out + t * p.o_stride + (int64_t) head * p.Dv;
 #pragma unroll
     for (int m = 0; m < NO; m++)
 #pragma unroll
         for (int b = 0; b < 4; b++) {
+            if (KW > 1 && m % KW != kg) continue;
             const int d = 32 * m + 8 * b + 4 * h;
             float y[4];
 #pragma unroll
@@ -728,16 +821,26 @@ pa_prompt_kernel(PromptParams p) {
         }
 }
 
-template <int TY, int DK, int DV>
-static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
-    // blocks of the launch: at most one more than whole ones for each prompt
-    const int64_t rows = (int64_t) p.T * p.gqa, per = ((int64_t) p.max_q * p.gqa + kPromptRows - 1) / kPromptRows;
-    const int64_t blocks = std::min(rows / kPromptRows + p.S, per * p.S) * p.Hkv;
+// Row blocks of `rows` rows that the launch may have: at most one more than whole ones for each prompt.
+static int64_t prompt_blocks(const PromptParams &p, int rows) {
+    const int64_t all = (int64_t) p.T * p.gqa, per = ((int64_t) p.max_q * p.gqa + rows - 1) / rows;
+    return std::min(all / rows + p.S, per * p.S) * p.Hkv;
+}
+
+template <int TY, int DK, int DV, bool VEC, int KW>
+static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
+    const int64_t blocks = prompt_blocks(p, PromptShape<TY, DK, DV, VEC, KW>::ROWS);
     if (blocks > (1 << 23)) return hipErrorInvalidValue;   // 256 threads each: a launch holds below 2^32
-    const dim3 grid((unsigned) blocks), wg(kPromptThreads);
-    if (vec) hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, true>), grid, wg, 0, stream, p);
-    else hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, false>), grid, wg, 0, stream, p);
+    hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, VEC, KW>), dim3((unsigned) blocks), dim3(kPromptThreads), 0, stream, p);
     return hipGetLastError();
+}
+
+// KWS: waves that share rows in a small call.
+template <int TY, int DK, int DV, int KWS>
+static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
+    if (!vec) return launch_prompt_k<TY, DK, DV, false, 1>(p, stream);
+    if (KWS > 1 && prompt_blocks(p, 128) <= kPromptSplitBlocks) return launch_prompt_k<TY, DK, DV, true, KWS>(p, stream);
+    return launch_prompt_k<TY, DK, DV, true, 1>(p, stream);
 }
 
 // Rows of whole aligned pieces of 16 bytes.

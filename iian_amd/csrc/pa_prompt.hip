@@ -6,10 +6,10 @@ namespace iian_pa {
 hipError_t launch_prompt_f16(const PromptParams &p, hipStream_t stream) {
     const bool vec = prompt_vec<1>(p);
     const int d = std::max(p.D, p.Dv);
-    if (d <= 64) return launch_prompt_d<1, 64, 64>(p, vec, stream);
-    if (d <= 96) return launch_prompt_d<1, 96, 96>(p, vec, stream);
-    if (d <= 128) return launch_prompt_d<1, 128, 128>(p, vec, stream);
-    return launch_prompt_d<1, 256, 256>(p, vec, stream);
+    if (d <= 64) return launch_prompt_d<1, 64, 64, 4>(p, vec, stream);
+    if (d <= 96) return launch_prompt_d<1, 96, 96, 4>(p, vec, stream);
+    if (d <= 128) return launch_prompt_d<1, 128, 128, 4>(p, vec, stream);
+    return launch_prompt_d<1, 256, 256, 2>(p, vec, stream);
 }
 
 hipError_t launch_prompt(const PromptParams &p, int type, hipStream_t stream) {

@@ -124,6 +124,20 @@ def one(pa, lens, H, Hkv, D, kind="bf16", Dv=None, causal=True, n_swa=0, softcap
     return q, k, v, out, qsl
 
 
+def image_ends(n, g):
+    e = torch.arange(1, n + 1)
+    a = 5
+    while a < n:
+        b = min(n, a + int(torch.randint(3, 120, (1,), generator=g)))
+        e[a:b] = b
+        a = b + int(torch.randint(1, 60, (1,), generator=g))
+    return e
+
+
+ENDS = {"images": image_ends, "any": lambda n, g: torch.randint(-5, n + 9, (n,), generator=g),
+        "none": lambda n, g: torch.zeros(n, dtype=torch.int64), "last_only": lambda n, g: (torch.arange(n) == n - 1) * n}
+
+
 LENS = [(1,), (1, 2, 3, 1), (16,), (31, 33), (63, 64, 65), (100, 1, 0, 257), (400, 129), (0, 5, 0, 0, 40)]
 
 
@@ -139,6 +153,36 @@ def test_lengths(pa, lens, kind, heads):
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
 def test_head_sizes(pa, D, Dv, kind):
     one(pa, (70, 150), 4, 2, D, Dv=Dv, kind=kind)
+
+
+MANY = [1 + 37 * i % 250 for i in range(45)]    # enough row blocks that no two waves share rows
+
+
+@pytest.mark.parametrize("D,Dv", [(64, 64), (48, 8), (80, 96), (128, 128), (128, 104), (256, 256), (136, 200)])
+@pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
+def test_many_prompts(pa, D, Dv, kind):
+    one(pa, MANY, 16, 8, D, Dv=Dv, kind=kind, lead=2, tail=3)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("kw", [
+    dict(causal=False), dict(n_swa=40), dict(causal=False, n_swa=70), dict(softcap=5.0), dict(scale=-0.1), dict(mult=6.0),
+    dict(fused=True, off=8), dict(images=True), dict(images=True, n_swa=50), dict(empty=True),
+], ids=str)
+def test_many_prompts_masked(pa, kw, kind):
+    ends = image_ends if kw.get("images") else ENDS["any"] if kw.get("empty") else None
+    one(pa, MANY, 16, 8, 128, kind=kind, ends=ends, **{k: v for k, v in kw.items() if k not in ("images", "empty")})
+
+
+@pytest.mark.parametrize("S,L", [(64, 30), (65, 30), (200, 9), (1500, 3), (5000, 1)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_counts(pa, S, L, causal):
+    """The order of the row blocks: up to 64 prompts, more, and more than 64 shares of 64."""
+    one(pa, [1 + (7 * i) % L for i in range(S)], 4, 4, 64, causal=causal, lead=1)
+
+
+def test_one_long_prompt(pa):
+    one(pa, (3000,), 8, 8, 64, kind="f16")
 
 
 @pytest.mark.parametrize("D,Dv,kind", [(1, 1, "f32"), (33, 33, "bf16"), (100, 100, "f16"), (128, 33, "bf16"), (320, 320, "f16"),
@@ -162,20 +206,6 @@ def test_masks_and_values(pa, kw, kind):
     one(pa, (300, 77, 223), 8, 2, 128, kind=kind, **kw)
 
 
-def image_ends(n, g):
-    e = torch.arange(1, n + 1)
-    a = 5
-    while a < n:
-        b = min(n, a + int(torch.randint(3, 120, (1,), generator=g)))
-        e[a:b] = b
-        a = b + int(torch.randint(1, 60, (1,), generator=g))
-    return e
-
-
-ENDS = {"images": image_ends, "any": lambda n, g: torch.randint(-5, n + 9, (n,), generator=g),
-        "none": lambda n, g: torch.zeros(n, dtype=torch.int64), "last_only": lambda n, g: (torch.arange(n) == n - 1) * n}
-
-
 @pytest.mark.parametrize("kind", ["bf16", "f32"])
 @pytest.mark.parametrize("ends", list(ENDS))
 @pytest.mark.parametrize("n_swa", [0, 40])
@@ -191,7 +221,8 @@ def test_unaligned_rows(pa, off, D, kind):
 
 @pytest.mark.parametrize("kind", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("what", ["nan", "inf", "big"])
-def test_hidden_values_reach_nothing(pa, kind, what):
+@pytest.mark.parametrize("H,Hkv", [(8, 2), (64, 32)])
+def test_hidden_values_reach_nothing(pa, kind, what, H, Hkv):
     """A later token's k and v, whatever they hold, leave the tokens before it alone."""
     bad = {"nan": float("nan"), "inf": float("inf"), "big": torch.finfo(DT[kind]).max}[what]
 
@@ -202,7 +233,7 @@ def test_hidden_values_reach_nothing(pa, kind, what):
             v[t, 0, 9] = -bad
     # rows from 40 on see one: compared up to there, and from the next prompt on
     g = torch.Generator().manual_seed(1)
-    q, k, v = rows(g, 300, 8, 2, 128, 128, kind)
+    q, k, v = rows(g, 300, H, Hkv, 128, 128, kind)
     qsl = torch.tensor([0, 200, 300], dtype=torch.int32, device="cuda")
     prm = pa.PagedAttnParams(scale=128 ** -0.5)
     clean = pa.prompt_attn(q, k, v, qsl, 200, prm).clone()
