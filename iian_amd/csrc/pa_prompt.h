@@ -45,7 +45,7 @@ namespace iian_pa {
 
 constexpr int kPromptWaves = 4;
 constexpr int kPromptThreads = kPromptWaves * 64;
-constexpr int kPromptSplitBlocks = 256;   // blocks of 128 rows up to which waves share rows
+constexpr int kPromptCus = 256;   // an MI355X
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
@@ -200,7 +200,17 @@ __device__ __forceinline__ float max_halves(float x) {
     return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
-// Zeroes the non-finite 16-bit values of a piece; whether there were any.
+// Whether a 16-bit piece holds non-finite values.
+template <int TY>
+__device__ __forceinline__ bool any_bad(const u32x4 &a) {
+    typedef uint16_t h2 __attribute__((ext_vector_type(2)));
+    constexpr uint32_t EXP = TY == 30 ? 0x7f807f80u : 0x7c007c00u;
+    auto e = [&](int i) { return __builtin_bit_cast(h2, a[i] & EXP); };
+    const h2 m = __builtin_elementwise_max(__builtin_elementwise_max(e(0), e(1)), __builtin_elementwise_max(e(2), e(3)));
+    return m[0] == (uint16_t) EXP || m[1] == (uint16_t) EXP;
+}
+
+// Zeroes the non-finite values of a piece; whether there were any.
 template <int TY>
 __device__ __forceinline__ bool finite_piece(Piece8<TY> &x) {
     bool bad = false;
@@ -244,11 +254,12 @@ struct PromptBlock {
 template <int ROWS>
 __device__ __forceinline__ bool find_block(const PromptParams &p, int b, PromptBlock &out) {
     const int lane = threadIdx.x & 63;
-    auto prompt = [&](int s, int &a, int &len) {
-        a = min(max(p.qsl[s], 0), p.T);
-        len = min(max(p.qsl[s + 1], a), p.T) - a;
-        return (int) (((int64_t) min(len, p.max_q) * p.gqa + ROWS - 1) / ROWS);
+    auto blocks = [&](int from, int to, int &a, int &len) {
+        a = min(max(from, 0), p.T);
+        len = min(max(to, a), p.T) - a;
+        return (int) ((uint32_t) (min(len, p.max_q) * p.gqa + ROWS - 1) / ROWS);   // (the host holds tokens times heads below 2^31)
     };
+    auto prompt = [&](int s, int &a, int &len) { return blocks(p.qsl[s], p.qsl[s + 1], a, len); };
     int a = 0, len = 0, n = 0, s0 = 0;
     if (p.S <= 64) {
         if (lane < p.S) n = prompt(lane, a, len);
@@ -256,10 +267,10 @@ __device__ __forceinline__ bool find_block(const PromptParams &p, int b, PromptB
             int at, rb;
             if (p.causal || p.row_end) {
                 // the largest row block index r with more than b blocks at r or above
-                int lo = 0, above = 0, hi = INT32_MAX;   // sum over prompts of max(0, n - lo) > b; at hi it is not
-                const int all = __builtin_amdgcn_readlane(lane_scan(n), 63);
-                if (b >= all) return false;
-                for (hi = all; hi - lo > 1;) {
+                // (the sum over prompts of max(0, n - lo) is above b, at hi it is not)
+                int lo = 0, above = 0, hi = (int) ((uint32_t) (p.max_q * p.gqa + ROWS - 1) / ROWS);
+                if (b >= __builtin_amdgcn_readlane(lane_scan(n), 63)) return false;
+                while (hi - lo > 1) {
                     const int m = (lo + hi) >> 1, c = __builtin_amdgcn_readlane(lane_scan(max(0, n - m)), 63);
                     if (c > b) lo = m;
                     else hi = m, above = c;
@@ -286,7 +297,14 @@ __device__ __forceinline__ bool find_block(const PromptParams &p, int b, PromptB
         // the lane's share of the prompts, then the prompts of the share that holds b
         const int per = (p.S + 63) / 64;
         int sum = 0;
-        for (int s = lane * per; s < min(p.S, (lane + 1) * per); s++) sum += prompt(s, a, len);
+        for (int s = lane * per, last = min(p.S, (lane + 1) * per); s < last; s += 8) {
+            int at[9];   // (together: one wait for the nine)
+#pragma unroll
+            for (int j = 0; j < 9; j++) at[j] = p.qsl[min(s + j, last)];
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (s + j < last) sum += blocks(at[j], at[j + 1], a, len);
+        }
         const int scan = lane_scan(sum);
         const uint64_t m = __ballot(scan > b);
         if (!m) return false;
@@ -341,15 +359,19 @@ __global__ __launch_bounds__(kPromptThreads)
     // ---- the wave's rows: token i of the lane's row, and the tokens it sees, [lo, end) ----
     const int row = row0 + n;
     const bool live = row < rows;
-    const int i = live ? row / p.gqa : 0, head = hk * p.gqa + (live ? row - i * p.gqa : 0);
+    // token of row r of the workgroup's: one division for all of them, the rest exact in fp32 (below 2^24)
+    const int base = wg0 / p.gqa, off = wg0 - base * p.gqa;
+    const float inv_gqa = 1.f / (float) p.gqa;
+    auto token_of = [&](int r) { return base + (int) (((float) (r - wg0 + off) + 0.5f) * inv_gqa); };
+    const int i = live ? token_of(row) : 0, head = hk * p.gqa + (live ? row - i * p.gqa : 0);
     const int64_t t = q0 + i;
     int end = 0;
     if (live) end = p.row_end ? min(max(p.row_end[t], 0), L) : p.causal ? i + 1 : L;
     const int lo = p.n_swa > 0 ? max(0, i - p.n_swa + 1) : 0;
     // of the wave: the tokens that all of its rows see, [w_lo_all, w_end_all), and that any sees, [w_lo, w_end)
-    const int last = min(row0 + 31, rows - 1), i_first = row0 / p.gqa, i_last = last / p.gqa;
+    const int i_first = token_of(row0), i_last = token_of(min(row0 + 31, rows - 1));
     // of the workgroup: its tiles start in [g_lo, g_end), and all of its rows see [g_lo_all, g_end_all)
-    const int g_first = wg0 / p.gqa, g_last = (min(wg0 + ROWS, rows) - 1) / p.gqa;
+    const int g_first = base, g_last = token_of(min(wg0 + ROWS, rows) - 1);
     int w_end, w_end_all, g_end, g_end_all;
     if (p.row_end) {
         int mx = end, mn = live ? end : INT32_MAX;
@@ -580,19 +602,22 @@ __global__ __launch_bounds__(kPromptThreads)
     auto tile = [&](int c0, auto buf_) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_)::value, ahead = (buf + NB - 1) % NB;   // ahead: the tile that is loaded meanwhile
         load_tile(c0 + (NB - 1) * TT, ahead);
-        if (DMA && partial(c0)) {
-            bool bad = false;
+        if constexpr (DMA) {
+            if (partial(c0)) {
+                char *const at = lds_v + buf * SH::BUF + tid * 16;
+                bool bad = false;
 #pragma unroll
-            for (int x = 0; x < SH::PPT; x++) {
-                Piece8<TY> v;
-                u32x4 *at = (u32x4 *) (lds_v + buf * SH::BUF + (tid + x * kPromptThreads) * 16);
-                if constexpr (!F32) {
-                    v.a = *at;
-                    if (finite_piece<TY>(v)) *at = v.a, bad = true;
+                for (int x = 0; x < SH::PPT; x++) bad |= any_bad<TY>(*(const u32x4 *) (at + x * kPromptThreads * 16));
+                if (bad) {
+                    for (int x = 0; x < SH::PPT; x++) {
+                        Piece8<TY> v = {*(const u32x4 *) (at + x * kPromptThreads * 16)};
+                        finite_piece<TY>(v);
+                        *(u32x4 *) (at + x * kPromptThreads * 16) = v.a;
+                    }
+                    bad_v = 1;
                 }
+                __syncthreads();
             }
-            if (bad) bad_v = 1;
-            __syncthreads();
         }
         const int cw = c0 + KT * kg;
         if (cw < w_end && cw + KT > w_lo) {   // wave-uniform: some row sees some of it
@@ -798,27 +823,65 @@ __global__ __launch_bounds__(kPromptThreads)
 
     // ---- rows out ----
     float inv = l == 0.f ? 0.f : 1.f / l;
-    if (!live) return;
     if constexpr (F32 && KW == 1) inv *= v_ref;   // (an empty row: 0 * 2^-126)
     T *out = (T *) p.out + t * p.o_stride + (int64_t) head * p.Dv;
+    if constexpr (VEC && KW == 1) {
+        // Through the wave's part of LDS (the tiles are read: the loop ended with a barrier), so that a store writes whole
+        // rows, 16 bytes a lane, instead of 4 values in each of 64 places.  128 bytes of the rows at a time.
+        constexpr int ES = sizeof(T), MB = 4 / ES, RB = 128 + 16, LPR = 8, RPI = 64 / LPR;   // row pitch, lanes per row, rows per store
+        static_assert(32 * RB * kPromptWaves <= sizeof(lds), "the rows fit");
+        char *const my = lds + wave * 32 * RB;
+        const int last = min(31, rows - 1 - row0);
+        // (a row's place: its own lane knows it)
+        const int64_t place = t * p.o_stride + (int64_t) head * p.Dv;
 #pragma unroll
-    for (int m = 0; m < NO; m++)
+        for (int m0 = 0; m0 < NO; m0 += MB) {
 #pragma unroll
-        for (int b = 0; b < 4; b++) {
-            if (KW > 1 && m % KW != kg) continue;
-            const int d = 32 * m + 8 * b + 4 * h;
-            float y[4];
+            for (int m = m0; m < (NO < m0 + MB ? NO : m0 + MB); m++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = o[m][4 * b + e] * inv;
-            if (VEC && d < p.Dv) {
-                if constexpr (F32) *(float4 *) (out + d) = make_float4(y[0], y[1], y[2], y[3]);
-                else *(u32x2 *) (out + d) = u32x2{pack2<TY>(y[0], y[1]), pack2<TY>(y[2], y[3])};
-            } else if (!VEC) {
+                for (int b = 0; b < 4; b++) {
+                    char *at = my + n * RB + (32 * (m - m0) + 8 * b + 4 * h) * ES;
+                    float y[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (d + e < p.Dv) out[d + e] = (T) y[e];
+                    for (int e = 0; e < 4; e++) y[e] = o[m][4 * b + e] * inv;
+                    if constexpr (F32) *(float4 *) at = make_float4(y[0], y[1], y[2], y[3]);
+                    else *(u32x2 *) at = u32x2{pack2<TY>(y[0], y[1]), pack2<TY>(y[2], y[3])};
+                }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int x = 0; x < 32 / RPI; x++) {
+                const int r = x * RPI + lane / LPR, d = 32 * m0 + lane % LPR * (16 / ES);
+                const int64_t to = __shfl(place, r);
+                const u32x4 y = *(const u32x4 *) (my + r * RB + lane % LPR * 16);
+                if (r <= last && d < p.Dv && d < 32 * NO) *(u32x4 *) ((T *) p.out + to + d) = y;
             }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
+    } else {
+        if (!live) return;
+#pragma unroll
+        for (int m = 0; m < NO; m++)
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                if (KW > 1 && m % KW != kg) continue;
+                const int d = 32 * m + 8 * b + 4 * h;
+                float y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = o[m][4 * b + e] * inv;
+                if (VEC && d < p.Dv) {
+                    if constexpr (F32) *(float4 *) (out + d) = make_float4(y[0], y[1], y[2], y[3]);
+                    else *(u32x2 *) (out + d) = u32x2{pack2<TY>(y[0], y[1]), pack2<TY>(y[2], y[3])};
+                } else if (!VEC) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (d + e < p.Dv) out[d + e] = (T) y[e];
+                }
+            }
+    }
 }
 
 // Row blocks of `rows` rows that the launch may have: at most one more than whole ones for each prompt.
@@ -835,11 +898,16 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// KWS: waves that share rows in a small call.
-template <int TY, int DK, int DV, int KWS>
+// KW4, KW2: whether waves may share rows by four, by two (LDS holds their tiles).
+// They do in calls whose workgroups then still run at once: one of KW = 4 fits a
+// CU, two of KW = 2.
+template <int TY, int DK, int DV, bool KW4, bool KW2>
 static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
     if (!vec) return launch_prompt_k<TY, DK, DV, false, 1>(p, stream);
-    if (KWS > 1 && prompt_blocks(p, 128) <= kPromptSplitBlocks) return launch_prompt_k<TY, DK, DV, true, KWS>(p, stream);
+    if constexpr (KW4)
+        if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4>(p, stream);
+    if constexpr (KW2)
+        if (prompt_blocks(p, 64) <= (KW4 ? 2 : 1) * kPromptCus) return launch_prompt_k<TY, DK, DV, true, 2>(p, stream);
     return launch_prompt_k<TY, DK, DV, true, 1>(p, stream);
 }
 

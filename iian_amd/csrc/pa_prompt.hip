@@ -6,14 +6,15 @@ namespace iian_pa {
 hipError_t launch_prompt_f16(const PromptParams &p, hipStream_t stream) {
     const bool vec = prompt_vec<1>(p);
     const int d = std::max(p.D, p.Dv);
-    if (d <= 64) return launch_prompt_d<1, 64, 64, 4>(p, vec, stream);
-    if (d <= 96) return launch_prompt_d<1, 96, 96, 4>(p, vec, stream);
-    if (d <= 128) return launch_prompt_d<1, 128, 128, 4>(p, vec, stream);
-    return launch_prompt_d<1, 256, 256, 2>(p, vec, stream);
+    if (d <= 64) return launch_prompt_d<1, 64, 64, true, true>(p, vec, stream);
+    if (d <= 96) return launch_prompt_d<1, 96, 96, true, true>(p, vec, stream);
+    if (d <= 128) return launch_prompt_d<1, 128, 128, true, true>(p, vec, stream);
+    return launch_prompt_d<1, 256, 256, false, true>(p, vec, stream);
 }
 
 hipError_t launch_prompt(const PromptParams &p, int type, hipStream_t stream) {
-    if (std::max(p.D, p.Dv) > 256) return launch_prompt_rows(p, type, stream);
+    // (token numbers within a workgroup come from an fp32 product)
+    if (std::max(p.D, p.Dv) > 256 || p.gqa > 65536) return launch_prompt_rows(p, type, stream);
     switch (type) {
         case 0: return launch_prompt_f32(p, stream);
         case 1: return launch_prompt_f16(p, stream);
