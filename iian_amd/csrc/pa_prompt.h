@@ -43,8 +43,6 @@
 
 namespace iian_pa {
 
-constexpr int kPromptWaves = 4;
-constexpr int kPromptThreads = kPromptWaves * 64;
 constexpr int kPromptCus = 256;   // an MI355X
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -66,19 +64,20 @@ struct PromptType<0> {
 };
 
 // TY: rows' type; DK: head size rounded up to 16 dims, DV: to 32; VEC: rows of
-// whole aligned 16-byte pieces; KW: waves that share their rows.
+// whole aligned 16-byte pieces; KW: waves that share their rows; NW: waves of a
+// workgroup.
 //
 // LDS tiles.  Rows are unpadded, so that tiles of 16-bit rows can be loaded
 // straight into LDS (16 consecutive bytes per lane), and the 16-byte pieces of
 // row r are permuted by an exclusive or with swz(r) instead: 16 rows read at one
 // piece, as QK^T does, and the 4 rows x 64 bytes of a transpose read each fill
 // the 64 banks.
-template <int TY, int DK, int DV, bool VEC, int KW>
+template <int TY, int DK, int DV, bool VEC, int KW, int NW>
 struct PromptShape {
     static constexpr int NP = TY == 0 ? 2 : 1;             // 16-bit terms per value
     static constexpr bool DMA = VEC && TY != 0;            // tiles go straight into LDS
     static constexpr int KT = 32, TT = KT * KW;            // tokens per wave and tile, and per workgroup's
-    static constexpr int ROWS = 32 * (kPromptWaves / KW);  // rows per workgroup
+    static constexpr int THREADS = NW * 64, ROWS = 32 * (NW / KW);   // of a workgroup
     static constexpr int KS = DK / 16, NO = DV / 32, NS = 16;
     static constexpr int CPR = DK <= 64 ? 8 : DK <= 128 ? 16 : 32;   // 16-byte pieces per row
     static_assert((DV <= 64 ? 8 : DV <= 128 ? 16 : 32) == CPR, "K and V rows of one pitch");
@@ -86,10 +85,13 @@ struct PromptShape {
     static constexpr int PLANE = TT * STRIDE, BUF = NP * PLANE;
     // three buffers (loads two tiles ahead) where three workgroups of them fit a CU's 160 KB of LDS
     static constexpr int NB = DMA && BUF * 6 <= 49152 ? 3 : 2;
-    static constexpr int PPT = TT * CPR / kPromptThreads;  // pieces per thread and tile
-    static_assert(PPT * kPromptThreads == TT * CPR, "pieces divide evenly");
+    static constexpr int PPT = TT * CPR / THREADS;  // pieces per thread and tile
+    static_assert(PPT * THREADS == TT * CPR, "pieces divide evenly");
+    // Q pieces (of KS) that wait in LDS instead of registers: with 8 waves of head size 256, O and half of Q fit the 256
+    // registers that two waves per SIMD have
+    static constexpr int QL = NW == 8 ? KS / 2 : 0;
     // waves per SIMD asked of the register allocator
-    static constexpr int WAVES = DK > 128 ? 1 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
+    static constexpr int WAVES = DK > 128 ? NW / 4 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
     __device__ static __forceinline__ int swz(int r) {
         return CPR == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -330,22 +332,23 @@ __device__ __forceinline__ bool find_block(const PromptParams &p, int b, PromptB
     }
 }
 
-template <int TY, int DK, int DV, bool VEC, int KW>
-__global__ __launch_bounds__(kPromptThreads)
-    __attribute__((amdgpu_waves_per_eu(PromptShape<TY, DK, DV, VEC, KW>::WAVES))) void pa_prompt_kernel(PromptParams p) {
-    using SH = PromptShape<TY, DK, DV, VEC, KW>;
+template <int TY, int DK, int DV, bool VEC, int KW, int NW>
+__global__ __launch_bounds__(NW * 64)
+    __attribute__((amdgpu_waves_per_eu(PromptShape<TY, DK, DV, VEC, KW, NW>::WAVES))) void pa_prompt_kernel(PromptParams p) {
+    using SH = PromptShape<TY, DK, DV, VEC, KW, NW>;
     using T = typename PromptType<TY>::T;
     constexpr bool F32 = TY == 0, DMA = SH::DMA;
     constexpr int NP = SH::NP, KT = SH::KT, TT = SH::TT, NB = SH::NB, KS = SH::KS, NO = SH::NO, NS = SH::NS, CPR = SH::CPR;
     constexpr int ROWS = SH::ROWS;
     // K and V tiles; in the end the waves' results that are joined
-    constexpr int JOIN = KW > 1 ? kPromptWaves * (NO * 16 + 2) * 64 * 4 : 0;
+    constexpr int JOIN = KW > 1 ? NW * (NO * 16 + 2) * 64 * 4 : 0;
     __shared__ __attribute__((aligned(16))) char lds[std::max(2 * NB * SH::BUF, JOIN)];
     char *const lds_k = lds, *const lds_v = lds + NB * SH::BUF;
     __shared__ __attribute__((aligned(16))) float k_up[NB][F32 ? TT : 1];   // F32: 2^(e - 15) of each K row
     __shared__ __attribute__((aligned(16))) float v_up[NB][F32 ? TT : 1];   // and of each V row
+    __shared__ __attribute__((aligned(16))) u32x4 q_lds[std::max(1, NW * SH::QL * 64)];   // each lane's own Q pieces
     __shared__ int bad_v;   // some tile that is not seen whole had non-finite values of V (left out of it)
-    __shared__ int wave_end[2][kPromptWaves];
+    __shared__ int wave_end[2][NW];
 
     const int hk = blockIdx.x % p.Hkv;
     PromptBlock blk;
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(kPromptThreads)
         __syncthreads();
         mx = 0, mn = INT32_MAX;
 #pragma unroll
-        for (int w = 0; w < kPromptWaves; w++) mx = max(mx, wave_end[0][w]), mn = min(mn, wave_end[1][w]);
+        for (int w = 0; w < NW; w++) mx = max(mx, wave_end[0][w]), mn = min(mn, wave_end[1][w]);
         g_end = __builtin_amdgcn_readfirstlane(mx);
         g_end_all = __builtin_amdgcn_readfirstlane(mn);
     } else {
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(kPromptThreads)
     const T *kb = (const T *) p.k + q0 * p.k_stride + (int64_t) hk * p.D;
     const T *vb = (const T *) p.v + q0 * p.v_stride + (int64_t) hk * p.Dv;
     const int pr0 = tid / CPR;   // a thread's pieces: rows pr0 + x * (threads / CPR), at one place of the row
-    auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (kPromptThreads / CPR); };
+    auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (SH::THREADS / CPR); };
     auto piece_dim = [&](int x, int D) __attribute__((always_inline)) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k), lv0 = lds_addr(lds_v);
     Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
@@ -424,12 +427,12 @@ __global__ __launch_bounds__(kPromptThreads)
         const T *from = base + c0 * stride;
         if (c0 + TT <= L) {
 #pragma unroll
-            for (int x = 0; x < SH::PPT; x++) lds_load16_at(from, vo[x], lds, x * kPromptThreads * 16);
+            for (int x = 0; x < SH::PPT; x++) lds_load16_at(from, vo[x], lds, x * SH::THREADS * 16);
         } else {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
                 const uint32_t r = min(piece_row(x), L - 1 - c0);
-                lds_load16_at(from, (r * (uint32_t) stride + piece_dim(x, D)) * 2, lds, x * kPromptThreads * 16);
+                lds_load16_at(from, (r * (uint32_t) stride + piece_dim(x, D)) * 2, lds, x * SH::THREADS * 16);
             }
         }
     };
@@ -486,7 +489,7 @@ __global__ __launch_bounds__(kPromptThreads)
             const bool part = partial(c0);
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
-                const int at = buf * SH::BUF + (tid + x * kPromptThreads) * 16, r = piece_row(x);
+                const int at = buf * SH::BUF + (tid + x * SH::THREADS) * 16, r = piece_row(x);
                 float up = 1.f;
                 if constexpr (F32) up = row_scale(ks[x], &k_up[buf][r]);
                 put_piece(ks[x], lds_k + at, up);
@@ -508,7 +511,9 @@ __global__ __launch_bounds__(kPromptThreads)
     if constexpr (NB == 3) load_tile(g_lo + TT, 1);
 
     // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
-    u32x4 qr[NP][KS];
+    constexpr int QL = SH::QL, QR = KS - QL;   // the last QL pieces in LDS
+    u32x4 qr[NP][QR];
+    u32x4 *const ql = q_lds + wave * QL * 64 + lane;
     // of the product; above zero, so that a masked score stays -inf (a scale of zero takes Q as zero instead)
     float cs = p.scale == 0.f ? 1.f : fabsf(p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e);
     {
@@ -517,9 +522,11 @@ __global__ __launch_bounds__(kPromptThreads)
             const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                qr[0][k] = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live).a;
+                u32x4 x = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live).a;
 #pragma unroll
-                for (int e = 0; e < 4; e++) qr[0][k][e] = p.scale == 0.f ? 0 : qr[0][k][e] ^ sign;
+                for (int e = 0; e < 4; e++) x[e] = p.scale == 0.f ? 0 : x[e] ^ sign;
+                if (k < QR) qr[0][k] = x;
+                else ql[(k - QR) * 64] = x;
             }
         } else {
             Piece8<0> x[KS];
@@ -551,7 +558,7 @@ __global__ __launch_bounds__(kPromptThreads)
         cs = fmaxf(cs, 1e-37f);
         // Q is here: no wait for it (and with it for the tile in flight) inside the loop
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < QR; k++) {
             asm volatile("" : "+v"(qr[0][k]));
             if constexpr (F32) asm volatile("" : "+v"(qr[NP - 1][k]));
         }
@@ -584,11 +591,12 @@ __global__ __launch_bounds__(kPromptThreads)
     // Operands are read two products ahead; the scheduling barriers keep the compiler from pulling each read down to its
     // product, where the wave would wait for it.
     constexpr int NQ = NO * (NS / 8);   // products (triples of them, F32) of a tile with V; KS with K
-    u32x4 kr[3][NP], vr[3][NP];
+    u32x4 kr[3][NP], vr[3][NP], qv[3];
     auto read_k = [&](int k, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < NP; e++)
             kr[k % 3][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE);
+        if (k >= QR) qv[k % 3] = ql[(k - QR) * 64];
     };
     auto read_v = [&](int q, int buf) __attribute__((always_inline)) {
         const int st = q / NO, m = q % NO;
@@ -607,12 +615,12 @@ __global__ __launch_bounds__(kPromptThreads)
                 char *const at = lds_v + buf * SH::BUF + tid * 16;
                 bool bad = false;
 #pragma unroll
-                for (int x = 0; x < SH::PPT; x++) bad |= any_bad<TY>(*(const u32x4 *) (at + x * kPromptThreads * 16));
+                for (int x = 0; x < SH::PPT; x++) bad |= any_bad<TY>(*(const u32x4 *) (at + x * SH::THREADS * 16));
                 if (bad) {
                     for (int x = 0; x < SH::PPT; x++) {
-                        Piece8<TY> v = {*(const u32x4 *) (at + x * kPromptThreads * 16)};
+                        Piece8<TY> v = {*(const u32x4 *) (at + x * SH::THREADS * 16)};
                         finite_piece<TY>(v);
-                        *(u32x4 *) (at + x * kPromptThreads * 16) = v.a;
+                        *(u32x4 *) (at + x * SH::THREADS * 16) = v.a;
                     }
                     bad_v = 1;
                 }
@@ -631,7 +639,7 @@ __global__ __launch_bounds__(kPromptThreads)
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 if (k + 2 < KS) read_k(k + 2, buf);
-                sc = prompt_mfma<TY>(kr[k % 3][0], qr[0][k], sc);
+                sc = prompt_mfma<TY>(kr[k % 3][0], k < QR ? qr[0][k < QR ? k : 0] : qv[k % 3], sc);
                 if constexpr (F32) {
                     sc = prompt_mfma<TY>(kr[k % 3][NP - 1], qr[0][k], sc);
                     sc = prompt_mfma<TY>(kr[k % 3][0], qr[NP - 1][k], sc);
@@ -829,7 +837,7 @@ __global__ __launch_bounds__(kPromptThreads)
         // Through the wave's part of LDS (the tiles are read: the loop ended with a barrier), so that a store writes whole
         // rows, 16 bytes a lane, instead of 4 values in each of 64 places.  128 bytes of the rows at a time.
         constexpr int ES = sizeof(T), MB = 4 / ES, RB = 128 + 16, LPR = 8, RPI = 64 / LPR;   // row pitch, lanes per row, rows per store
-        static_assert(32 * RB * kPromptWaves <= sizeof(lds), "the rows fit");
+        static_assert(32 * RB * NW <= sizeof(lds), "the rows fit");
         char *const my = lds + wave * 32 * RB;
         const int last = min(31, rows - 1 - row0);
         // (a row's place: its own lane knows it)
@@ -890,25 +898,29 @@ static int64_t prompt_blocks(const PromptParams &p, int rows) {
     return std::min(all / rows + p.S, per * p.S) * p.Hkv;
 }
 
-template <int TY, int DK, int DV, bool VEC, int KW>
+template <int TY, int DK, int DV, bool VEC, int KW, int NW>
 static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
-    const int64_t blocks = prompt_blocks(p, PromptShape<TY, DK, DV, VEC, KW>::ROWS);
+    const int64_t blocks = prompt_blocks(p, PromptShape<TY, DK, DV, VEC, KW, NW>::ROWS);
     if (blocks > (1 << 23)) return hipErrorInvalidValue;   // 256 threads each: a launch holds below 2^32
-    hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, VEC, KW>), dim3((unsigned) blocks), dim3(kPromptThreads), 0, stream, p);
+    hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, VEC, KW, NW>), dim3((unsigned) blocks), dim3(NW * 64), 0, stream, p);
     return hipGetLastError();
 }
 
 // KW4, KW2: whether waves may share rows by four, by two (LDS holds their tiles).
 // They do in calls whose workgroups then still run at once: one of KW = 4 fits a
 // CU, two of KW = 2.
-template <int TY, int DK, int DV, bool KW4, bool KW2>
+//
+// NW8: whether the workgroups of the largest calls have 8 waves (head size 256).
+template <int TY, int DK, int DV, bool KW4, bool KW2, bool NW8 = false>
 static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
-    if (!vec) return launch_prompt_k<TY, DK, DV, false, 1>(p, stream);
+    if (!vec) return launch_prompt_k<TY, DK, DV, false, 1, 4>(p, stream);
     if constexpr (KW4)
-        if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4>(p, stream);
+        if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4, 4>(p, stream);
     if constexpr (KW2)
-        if (prompt_blocks(p, 64) <= (KW4 ? 2 : 1) * kPromptCus) return launch_prompt_k<TY, DK, DV, true, 2>(p, stream);
-    return launch_prompt_k<TY, DK, DV, true, 1>(p, stream);
+        if (prompt_blocks(p, 64) <= (KW4 ? 2 : 1) * kPromptCus) return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
+    if constexpr (NW8)
+        if (prompt_blocks(p, 256) > kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
+    return launch_prompt_k<TY, DK, DV, true, 1, 4>(p, stream);
 }
 
 // Rows of whole aligned pieces of 16 bytes.
