@@ -89,7 +89,7 @@ struct PromptShape {
     static_assert(PPT * THREADS == TT * CPR, "pieces divide evenly");
     // Q pieces (of KS) that wait in LDS instead of registers: with 8 waves of head size 256, O and half of Q fit the 256
     // registers that two waves per SIMD have
-    static constexpr int QL = NW == 8 ? KS / 2 : 0;
+    static constexpr int QL = NW == 8 ? KS * 5 / 8 : 0;
     // waves per SIMD asked of the register allocator
     static constexpr int WAVES = DK > 128 ? NW / 4 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
     __device__ static __forceinline__ int swz(int r) {
