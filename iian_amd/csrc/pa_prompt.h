@@ -423,24 +423,25 @@ __global__ __launch_bounds__(NW * 64)
     }
     const uint32_t lkw = __builtin_amdgcn_readfirstlane(lk0 + wave * 1024), lvw = __builtin_amdgcn_readfirstlane(lv0 + wave * 1024);
     // Rows c0 .. of a tile into LDS, or registers; nothing from g_end on.
-    auto load_rows = [&](const T *base, int64_t stride, const uint32_t (&vo)[SH::PPT], uint32_t lds, int D, int c0) __attribute__((always_inline)) {
-        const T *from = base + c0 * stride;
-        if (c0 + TT <= L) {
-#pragma unroll
-            for (int x = 0; x < SH::PPT; x++) lds_load16_at(from, vo[x], lds, x * SH::THREADS * 16);
-        } else {
-#pragma unroll
-            for (int x = 0; x < SH::PPT; x++) {
-                const uint32_t r = min(piece_row(x), L - 1 - c0);
-                lds_load16_at(from, (r * (uint32_t) stride + piece_dim(x, D)) * 2, lds, x * SH::THREADS * 16);
-            }
-        }
-    };
     auto load_tile = [&](int c0, int buf) __attribute__((always_inline)) {
         if (c0 >= g_end) return;
         if constexpr (DMA) {
-            load_rows(kb, p.k_stride, kvo, lkw + buf * SH::BUF, p.D, c0);
-            load_rows(vb, p.v_stride, vvo, lvw + buf * SH::BUF, p.Dv, c0);
+            const T *const kt = kb + c0 * p.k_stride, *const vt = vb + c0 * p.v_stride;
+            const uint32_t lk = lkw + buf * SH::BUF, lv = lvw + buf * SH::BUF;
+            if (c0 + TT <= L) {
+#pragma unroll
+                for (int x = 0; x < SH::PPT; x++) {
+                    lds_load16_at(kt, kvo[x], lk, x * SH::THREADS * 16);
+                    lds_load16_at(vt, vvo[x], lv, x * SH::THREADS * 16);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < SH::PPT; x++) {
+                    const uint32_t r = min(piece_row(x), L - 1 - c0);
+                    lds_load16_at(kt, (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2, lk, x * SH::THREADS * 16);
+                    lds_load16_at(vt, (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2, lv, x * SH::THREADS * 16);
+                }
+            }
         } else {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
@@ -577,14 +578,15 @@ __global__ __launch_bounds__(NW * 64)
     // exclusive or does not mix with the constants added, so a base per distinct pattern is kept: swz(n) is K's; rows r and
     // r + 8 (r + 16 is r again) are V's.
     const int vrow = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    // (opaque: kept as they are, so that what is added below is a constant of the read)
     uint32_t koff[KS], voff[2][NO];
 #pragma unroll
-    for (int k = 0; k < KS; k++) koff[k] = lk0 + (KT * kg + n) * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n));
+    for (int k = 0; k < KS; k++) koff[k] = opaque(lk0 + (KT * kg + n) * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n)));
 #pragma unroll
     for (int e = 0; e < 2; e++)
 #pragma unroll
         for (int m = 0; m < NO; m++)
-            voff[e][m] = lv0 + (KT * kg + vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1);
+            voff[e][m] = opaque(lv0 + (KT * kg + vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1));
 
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     // ---- the tile loop ----
