@@ -152,15 +152,45 @@ __device__ __forceinline__ int split_exp(float mx) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t) (127 + e) << 23); }
 
-// x = hi + lo to 22 bits, each rounded to nearest.  (The difference's terms pass
-// through empty asm: folded into a mixed-precision FMA with a negated operand it
-// has come out wrong, see split_f16x8.)
-__device__ __forceinline__ void split2(float x, _Float16 &hi, _Float16 &lo) {
-    asm volatile("" : "+v"(x));
-    hi = (_Float16) x;
-    float f = (float) hi;
-    asm volatile("" : "+v"(f));
-    lo = (_Float16) (x - f);
+// The larger of lanes l and l ^ 32.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+
+// x[2i], x[2i+1] = hi + lo to 22 bits, each rounded to nearest, into element i of
+// hi and lo (packed f16).  (The differences' terms pass through empty asm: folded
+// into a mixed-precision FMA with a negated operand they have come out wrong,
+// see split_f16x8.)
+__device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    asm volatile("" : "+v"(x0), "+v"(x1));
+    const h2 h = __builtin_convertvector((f2){x0, x1}, h2);
+    float f0 = (float) h[0], f1 = (float) h[1];
+    asm volatile("" : "+v"(f0), "+v"(f1));
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){x0 - f0, x1 - f1}, h2));
+}
+
+// Largest |x| of a piece, and of the pieces of CPR neighbouring lanes.
+__device__ __forceinline__ float piece_max(const Piece8<0> &x) {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+    return m;
+}
+template <int CPR>
+__device__ __forceinline__ float lanes_max(float m) {
+    auto with = [&](auto ctrl) __attribute__((always_inline)) {
+        return fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), decltype(ctrl)::value, 0xf, 0xf, true)));
+    };
+    m = with(std::integral_constant<int, 0xb1>());    // quad_perm [1, 0, 3, 2]
+    m = with(std::integral_constant<int, 0x4e>());    // quad_perm [2, 3, 0, 1]
+    m = with(std::integral_constant<int, 0x141>());   // row_half_mirror: the other quad of 8 lanes
+    if constexpr (CPR >= 16) m = with(std::integral_constant<int, 0x140>());   // row_mirror: the other 8 of 16
+    if constexpr (CPR >= 32) m = fmaxf(m, __shfl_xor(m, 16));
+    return m;
 }
 
 template <int TY>
@@ -194,12 +224,6 @@ __device__ __forceinline__ float sum2(uint32_t x, float c) {
         typedef _Float16 h2 __attribute__((ext_vector_type(2)));
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), (h2){(_Float16) 1.f, (_Float16) 1.f}, c, false);
     }
-}
-
-// The larger of lanes l and l ^ 32.
-__device__ __forceinline__ float max_halves(float x) {
-    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
 }
 
 // Whether a 16-bit piece holds non-finite values.
@@ -453,29 +477,24 @@ __global__ __launch_bounds__(NW * 64)
     };
     // F32: the scale of a row's pieces, which are in CPR neighbouring lanes
     auto row_scale = [&](const Piece8<TY> &x, float *up) __attribute__((always_inline)) {
-        float m = 0.f;
-        if constexpr (F32) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
-#pragma unroll
-            for (int o = 1; o < CPR; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-        }
-        const int ex = split_exp(m);
+        int ex = 0;
+        if constexpr (F32) ex = split_exp(lanes_max<CPR>(piece_max(x)));
         if (tid % CPR == 0) *up = pow2(ex - 15);
         return pow2(15 - ex);
     };
     auto put_piece = [&](const Piece8<TY> &x, char *at, float up) __attribute__((always_inline)) {
         if constexpr (F32) {
-            f16x8 hi, lw;
+            u32x4 hi, lw;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                _Float16 a, b;
-                split2((e < 4 ? x.a[e] : x.b[e - 4]) * up, a, b);
+            for (int e = 0; e < 4; e++) {
+                const f32x4 &y = e < 2 ? x.a : x.b;
+                uint32_t a, b;
+                split2(y[2 * (e & 1)] * up, y[2 * (e & 1) + 1] * up, a, b);
                 hi[e] = a;
                 lw[e] = b;
             }
-            *(f16x8 *) at = hi;
-            *(f16x8 *) (at + SH::PLANE) = lw;
+            *(u32x4 *) at = hi;
+            *(u32x4 *) (at + SH::PLANE) = lw;
         } else {
             *(u32x4 *) at = x.a;
         }
@@ -535,26 +554,21 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 x[k] = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live);
-#pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, fmaxf(fabsf(x[k].a[e]), fabsf(x[k].b[e])));
+                mx = fmaxf(mx, piece_max(x[k]));
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const int ex = split_exp(mx);
+            const int ex = split_exp(max_halves(mx));
             const float up = p.scale == 0.f ? 0.f : p.scale < 0.f ? -pow2(15 - ex) : pow2(15 - ex);
             cs *= pow2(ex - 15);
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                f16x8 hi, lw;
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    _Float16 a, b;
-                    split2((e < 4 ? x[k].a[e] : x[k].b[e - 4]) * up, a, b);
-                    hi[e] = a;
-                    lw[e] = b;
+                for (int e = 0; e < 4; e++) {
+                    const f32x4 &y = e < 2 ? x[k].a : x[k].b;
+                    uint32_t a, b;
+                    split2(y[2 * (e & 1)] * up, y[2 * (e & 1) + 1] * up, a, b);
+                    qr[0][k][e] = a;
+                    qr[NP - 1][k][e] = b;
                 }
-                qr[0][k] = __builtin_bit_cast(u32x4, hi);
-                qr[NP - 1][k] = __builtin_bit_cast(u32x4, lw);
-            }
         }
         cs = fmaxf(cs, 1e-37f);
         // Q is here: no wait for it (and with it for the tile in flight) inside the loop
@@ -699,10 +713,13 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
                     vf[j] = v_up[buf][KT * kg + 8 * (j / 4) + 4 * h + j % 4];
-                    top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
+                    top = fmaxf(top, vf[j]);
                 }
-                top = max_halves(top);
-                if (__any(top > v_ref * 64.f)) {
+                if (__any(top > v_ref * 64.f)) {   // (of all the tile's tokens: seldom)
+                    top = 0.f;
+#pragma unroll
+                    for (int j = 0; j < NS; j++) top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
+                    top = max_halves(top);
                     const float vn = top > v_ref * 64.f ? top : v_ref;
                     const float beta = v_ref / vn;
                     v_ref = vn;
@@ -711,21 +728,18 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
                         for (int r = 0; r < 16; r++) o[m][r] *= beta;
                 }
-                const float inv = 1.f / v_ref;
+                const float inv = 1.f / v_ref;   // a power of two
 #pragma unroll
-                for (int st = 0; st < NS / 8; st++) {
-                    f16x8 hi, lw;
+                for (int st = 0; st < NS / 8; st++)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        _Float16 a, b;
-                        // (a token of no weight may have any factor)
-                        split2(x[8 * st + e] != 0.f ? x[8 * st + e] * (vf[8 * st + e] * inv) : 0.f, a, b);
-                        hi[e] = a;
-                        lw[e] = b;
+                    for (int e = 0; e < 4; e++) {
+                        // (a token of no weight may have any factor: kept finite)
+                        const int j = 8 * st + 2 * e;
+                        uint32_t a, b;
+                        split2(x[j] * fminf(vf[j] * inv, 0x1p100f), x[j + 1] * fminf(vf[j + 1] * inv, 0x1p100f), a, b);
+                        pr[0][st][e] = a;
+                        pr[NP - 1][st][e] = b;
                     }
-                    pr[0][st] = __builtin_bit_cast(u32x4, hi);
-                    pr[NP - 1][st] = __builtin_bit_cast(u32x4, lw);
-                }
             }
             // ---- O^T += V^T P^T, the next 16 tokens' probabilities beside the products of 16 ----
             // (the sum is of the rounded probabilities, as the products are)
@@ -820,13 +834,15 @@ __global__ __launch_bounds__(NW * 64)
             if (!partial(j / TT * TT)) continue;
             const T *vr = vb + (int64_t) j * p.v_stride;
             const bool sees = j >= lo && j < end;
+            int Dv = p.Dv;   // (opaque: a comparison per value held over the whole kernel would take all scalar registers)
+            asm volatile("" : "+s"(Dv));
 #pragma unroll
             for (int m = 0; m < NO; m++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     if (KW > 1 && m % KW != kg) continue;
                     const int d = 32 * m + 8 * (r / 4) + 4 * h + r % 4;
-                    const float v = sees && d < p.Dv ? (float) vr[d] : 0.f;
+                    const float v = sees && d < Dv ? (float) vr[d] : 0.f;
                     o[m][r] += (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.f;
                 }
         }
