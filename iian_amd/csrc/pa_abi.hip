@@ -58,6 +58,7 @@ constexpr int kQ8DecodeWavesPerCu = 8;
 constexpr int kMaxWavesPerCu = kQ8DecodeWavesPerCu;
 constexpr int kDefaultCus = 256;   // an MI355X, when the device cannot be queried
 constexpr int kMaxHeadDim = 1024;  // largest head size the general kernel stages (pa_general.hip)
+constexpr int kMaxSeqs = 1 << 23;             // of the multi-axis positions and whole-prompt attention: a workgroup each stays within a launch's 2^32 threads
 constexpr int kMaxPromptTokens = 1 << 30;   // iian_pa_prompt_attention counts tokens and tiles past them in 32 bits
 constexpr int kMaxDevices = 64;
 
@@ -897,7 +898,7 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
 int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
                             const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
                             int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag) {
-    if (n_seqs < 0 || n_tokens < 0 || n_spans < 0) return IIAN_PA_ERR_ARG;
+    if (n_seqs < 0 || n_seqs > kMaxSeqs || n_tokens < 0 || n_spans < 0) return IIAN_PA_ERR_ARG;
     if (n_seqs == 0 || n_tokens == 0) return IIAN_PA_OK;
     if ((n_spans > 0 && !spans) || !span_off || !num_computed || !query_start_loc || !pos) return IIAN_PA_ERR_NULL;
     if ((uintptr_t) spans & 15) return IIAN_PA_ERR_ARG;   // a run is one 16-byte load
@@ -1063,7 +1064,7 @@ int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const v
                              int32_t n_head, int32_t n_head_kv, int32_t head_dim, int32_t head_dim_v, float scale,
                              float softcap, int32_t causal, int32_t n_swa, void *out, int64_t out_stride,
                              int32_t *err_flag) {
-    if (n_tokens < 0 || n_seqs < 0 || max_query_len < 0) return IIAN_PA_ERR_ARG;
+    if (n_tokens < 0 || n_seqs < 0 || n_seqs > kMaxSeqs || max_query_len < 0) return IIAN_PA_ERR_ARG;
     if (n_tokens == 0 || n_seqs == 0) return IIAN_PA_OK;
     if (!q || !k || !v || !query_start_loc || !out) return IIAN_PA_ERR_NULL;
     if (n_head <= 0 || n_head_kv <= 0 || n_head % n_head_kv || head_dim <= 0 || head_dim_v <= 0 ||

@@ -910,8 +910,10 @@ __global__ __launch_bounds__(NW * 64)
     }
 }
 
+constexpr int64_t kPromptMaxBlocks = 1 << 22;   // of at most 512 threads: a launch holds below 2^32
+
 // Row blocks of `rows` rows that the launch may have: at most one more than whole ones for each prompt.
-static int64_t prompt_blocks(const PromptParams &p, int rows) {
+inline int64_t prompt_blocks(const PromptParams &p, int rows) {
     const int64_t all = (int64_t) p.T * p.gqa, per = ((int64_t) p.max_q * p.gqa + rows - 1) / rows;
     return std::min(all / rows + p.S, per * p.S) * p.Hkv;
 }
@@ -919,7 +921,6 @@ static int64_t prompt_blocks(const PromptParams &p, int rows) {
 template <int TY, int DK, int DV, bool VEC, int KW, int NW>
 static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
     const int64_t blocks = prompt_blocks(p, PromptShape<TY, DK, DV, VEC, KW, NW>::ROWS);
-    if (blocks > (1 << 23)) return hipErrorInvalidValue;   // 256 threads each: a launch holds below 2^32
     hipLaunchKernelGGL((pa_prompt_kernel<TY, DK, DV, VEC, KW, NW>), dim3((unsigned) blocks), dim3(NW * 64), 0, stream, p);
     return hipGetLastError();
 }
@@ -947,7 +948,7 @@ static bool prompt_vec(const PromptParams &p) {
     const int64_t es = TY == 0 ? 4 : 2;
     const uintptr_t al = (uintptr_t) p.q | (uintptr_t) p.k | (uintptr_t) p.v | (uintptr_t) p.out;
     // (a tile's rows are addressed by 32-bit offsets)
-    if (std::max(p.k_stride, p.v_stride) >= 1 << 24) return false;
+    if (std::max(p.k_stride, p.v_stride) > 1 << 22) return false;
     return al % 16 == 0 && ((p.q_stride | p.k_stride | p.v_stride | p.o_stride) * es) % 16 == 0 && p.D % 8 == 0 && p.Dv % 8 == 0;
 }
 

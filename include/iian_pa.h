@@ -325,7 +325,8 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
  * memory.  *err_flag (when non-NULL) bit 3: a negative count or size, a grid
  * with h or w zero or a step below 1 (its tokens then count as none, its step
  * as 1), offsets out of order or outside [0, n_spans], or a position or end
- * past INT32_MAX, which is held there. */
+ * past INT32_MAX, which is held there; seen in the runs that the step's tokens
+ * need, those up to them.  At most 2^23 requests. */
 int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
                             const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
                             int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag);
@@ -406,7 +407,9 @@ int iian_pa_mrope_kv_write(void *stream, const iian_pa_mrope_rows *rows, const i
  * to [0, prompt length]), else i + 1 (causal) or the prompt's length.  A
  * token that sees none gets a zero row.  Rows outside every prompt are neither
  * read nor written.  A value of k or v that a token does not see never reaches
- * its output, infinities and NaN included.
+ * its output, infinities and NaN included (an infinity that an F32 token does
+ * see may make its output NaN).  out may be q itself with the same stride and
+ * head sizes, and must not overlap k or v.
  *   q [T][n_head][head_dim], k [T][n_head_kv][head_dim], v [T][n_head_kv][head_dim_v],
  *   out [T][n_head][head_dim_v], all of `type` (F32, F16 or BF16), tokens of
  *   q, k, v and out *_stride elements apart; aligned to their element
@@ -414,7 +417,8 @@ int iian_pa_mrope_kv_write(void *stream, const iian_pa_mrope_rows *rows, const i
  *                  longer one past it may be left unwritten and set bit 2 of *err_flag
  * Scores, sums and softmax statistics are fp32; F16 and BF16 rows enter the
  * matrix products as they are and probabilities rounded to their type, F32
- * rows as pairs of f16 terms (22 bits).  Head sizes 1 to 1024.  No workspace. */
+ * rows as pairs of f16 terms (22 bits).  Head sizes 1 to 1024, at most 2^23
+ * prompts, n_tokens * n_head below 2^31.  No workspace. */
 int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const void *v, int type, int64_t q_stride,
                              int64_t k_stride, int64_t v_stride, const int32_t *query_start_loc,
                              const int32_t *row_end, int32_t n_tokens, int32_t n_seqs, int32_t max_query_len,

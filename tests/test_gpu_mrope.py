@@ -335,3 +335,70 @@ def test_refusals(pa):
                 dict(k_rows=k.cpu()), dict(k_pool=pa.KVPool(8, 128, F16)), dict(q=k, q_out=torch.empty(4, 2, 32, device="cuda"))):
         with pytest.raises(ValueError):
             call(**bad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [128, 66])
+def test_offsets_past_32_bits(pa, D):
+    """Pool rows past 2^32 elements, and tokens far apart."""
+    T, Hkv = 70, 8
+    cells = (1 << 32) // (Hkv * D) + 4000
+    pool = torch.empty(cells, 2 * Hkv * D, dtype=torch.uint8, device="cuda")
+    kp, vp = pa.KVPool.wrap(pool, Hkv * D, F16), pa.KVPool(cells, Hkv, F16)
+    rows = torch.empty(T, (1 << 26) + 64, dtype=torch.float16, device="cuda")[:, :Hkv * D].view(T, Hkv, D)
+    rows.copy_(torch.randn(T, Hkv, D))
+    v = torch.randn(T, Hkv, 1, device="cuda").half()
+    slots = torch.arange(cells - T, cells, device="cuda")
+    pos = torch.randint(0, 9999, (2, T), dtype=torch.int32, device="cuda")
+    fr = torch.rand(D // 2, dtype=torch.float64, device="cuda")
+    ax = torch.randint(0, 2, (D // 2,), dtype=torch.int32, device="cuda")
+    ko = torch.empty(T, Hkv, D, dtype=torch.float16, device="cuda")
+    pa.mrope_set_rows_kv(kp, vp, rows, v, slots, pos, fr, ax, k_out=ko)
+    want, mag = rotated(rows, None, 0, pos, fr.cpu().numpy(), ax.cpu().numpy().astype(int), True, 1.0)
+    check(ko, want, mag, "f16")
+    assert torch.equal(kp.view_f16()[cells - T:], ko.view(T, -1))
+    assert torch.equal(vp.view_f16()[cells - T:], v.view(T, -1))
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs(pa):
+    """Positions and the write captured together, replayed with new inputs between eager work, and on two streams at once."""
+    T, H, Hkv, D = 60, 8, 2, 128
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(T, h, D, generator=g).bfloat16().cuda() for h in (H, Hkv, Hkv))
+    spans = cu([[9, 0, 0, 1], [2, 3, 4, 1], [7, 0, 0, 1]], torch.int32)
+    off, qsl = cu([0, 3], torch.int32), cu([0, T], torch.int32)
+    fr, ax, ms = pa.mrope_frequencies(pa.RopeParams(n_dims=D, freq_base=1e6), (16, 24, 24))
+    slots = torch.randperm(T + 4, generator=g)[:T].cuda()
+
+    def step(computed):
+        pos = torch.empty(3, T, dtype=torch.int32, device="cuda")
+        kp, vp = pa.KVPool(T + 4, Hkv * D, F16), pa.KVPool(T + 4, Hkv * D, F16)
+        qo = torch.empty_like(q)
+        return pos, kp, vp, qo, computed
+
+    def run(s):
+        pa.mrope_positions(spans, off, s[4], qsl, s[0])
+        pa.mrope_set_rows_kv(s[1], s[2], k, v, slots, s[0], fr, ax, q=q, q_out=s[3], mscale=ms)
+
+    computed = cu([5], torch.int32)
+    eager, captured = step(computed), step(computed)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(captured)
+    for n in (0, 3, 900):
+        computed.fill_(n)
+        run(eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eager[0], captured[0]) and torch.equal(eager[3], captured[3])
+        assert torch.equal(eager[1].data, captured[1].data) and torch.equal(eager[2].data, captured[2].data)
+        captured[3].zero_()
+    both = [step(computed), step(computed)]
+    torch.cuda.synchronize()
+    for s in both:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                run(s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(s[3], eager[3]) and torch.equal(s[1].data, eager[1].data) for s in both)

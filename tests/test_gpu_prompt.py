@@ -308,3 +308,72 @@ def test_refusals(pa):
             pa.prompt_attn(q, k, k, qsl, n, prm)
     with pytest.raises(pa.PagedAttnError):
         pa.prompt_attn(q[:, :3].contiguous(), k, k, qsl, 4, prm)
+
+
+def test_out_in_place_of_q(pa):
+    for kind, H, n in (("bf16", 8, 300), ("f32", 64, 900)):
+        q, k, v = rows(torch.Generator().manual_seed(5), n, H, H // 4, 128, 128, kind)
+        qsl = torch.tensor([0, n // 3, n], dtype=torch.int32, device="cuda")
+        prm = pa.PagedAttnParams(scale=128 ** -0.5)
+        want = pa.prompt_attn(q, k, v, qsl, n, prm)
+        pa.prompt_attn(q, k, v, qsl, n, prm, out=q)
+        assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_offsets_past_32_bits(pa, kind):
+    """Tokens far apart: element offsets of the last ones past 2^32."""
+    T, H, Hkv, D = 1100, 4, 1, 64
+    stride = 4000000                     # (16-bit rows: addressed per tile; the unaligned form's addresses are 64-bit)
+    dt = DT[kind]
+    g = torch.Generator().manual_seed(6)
+    buf = torch.empty(T * stride, dtype=dt, device="cuda")
+    x = buf.view(T, stride)[:, :(H + 2 * Hkv) * D]
+    x.copy_(torch.randn(T, (H + 2 * Hkv) * D, generator=g))
+    q, k, v = (t.unflatten(1, (n, D)) for t, n in zip(x.split((H * D, Hkv * D, Hkv * D), 1), (H, Hkv, Hkv)))
+    qsl = torch.tensor([0, 500, T], dtype=torch.int32, device="cuda")
+    prm = pa.PagedAttnParams(scale=0.125)
+    far = pa.prompt_attn(q, k, v, qsl, T, prm)
+    assert torch.equal(far, pa.prompt_attn(q.contiguous(), k.contiguous(), v.contiguous(), qsl, T, prm))
+    d = definition(q[500:], k[500:], v[500:], (T - 500,), 0.125)
+    assert ((far[500:].double().cpu() - d[0]).abs() <= tolerance(kind, D, *d)).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_streams_and_graphs(pa, kind):
+    """Two calls at once on two streams, and a captured call replayed with new inputs between eager work."""
+    prm = pa.PagedAttnParams(scale=128 ** -0.5)
+    sets = []
+    for n, H in ((700, 32), (90, 8)):
+        q, k, v = rows(torch.Generator().manual_seed(n), n, H, H // 4, 128, 128, kind)
+        qsl = torch.tensor([0, n // 2, n], dtype=torch.int32, device="cuda")
+        sets.append((q, k, v, qsl, n, pa.prompt_attn(q, k, v, qsl, n, prm)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for st, (q, k, v, qsl, n, _) in zip(streams, sets):
+        with torch.cuda.stream(st):
+            got.append([pa.prompt_attn(q, k, v, qsl, n, prm) for _ in range(5)])
+    torch.cuda.synchronize()
+    for g, s in zip(got, sets):
+        assert all(torch.equal(y, s[5]) for y in g)
+    for q, k, v, qsl, n, want in sets:
+        out = torch.zeros_like(want)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pa.prompt_attn(q, k, v, qsl, n, prm, out=out)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            k.mul_(-1)
+            want = pa.prompt_attn(q, k, v, qsl, n, prm)
+            out.zero_()
+
+
+def test_the_same_call_gives_the_same_bits(pa):
+    q, k, v = rows(torch.Generator().manual_seed(8), 2000, 16, 4, 128, 128, "f16")
+    qsl = torch.tensor([0, 3, 1200, 2000], dtype=torch.int32, device="cuda")
+    prm = pa.PagedAttnParams(scale=128 ** -0.5)
+    a = [pa.prompt_attn(q, k, v, qsl, 1997, prm) for _ in range(4)]
+    assert all(torch.equal(a[0], x) for x in a[1:])
