@@ -1099,6 +1099,7 @@ int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const v
     p.H = n_head;
     p.Hkv = n_head_kv;
     p.gqa = n_head / n_head_kv;
+    p.gqa_mul = p.gqa > 1 ? (uint32_t) (((uint64_t) 1 << 32) / p.gqa + 1) : 0;
     p.D = head_dim;
     p.Dv = head_dim_v;
     p.scale = scale;

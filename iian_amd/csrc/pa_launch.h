@@ -171,6 +171,7 @@ struct PromptParams {
     int32_t T, S, max_q, H, Hkv, gqa, D, Dv;
     float scale, softcap;
     int32_t causal, n_swa;
+    uint32_t gqa_mul;             // 2^32 / gqa + 1 (0 for gqa = 1): division by gqa on the device
 };
 // Matrix-core kernels at head sizes up to 256, the row form above (pa_prompt.hip).
 hipError_t launch_prompt(const PromptParams &p, int type, hipStream_t stream);

@@ -257,6 +257,14 @@ __device__ __forceinline__ bool finite_piece(Piece8<TY> &x) {
     return bad;
 }
 
+// r / gqa by the host's multiplier (2^32 / gqa + 1: at most one too many for r
+// below 2^31; 0 for gqa = 1).
+__device__ __forceinline__ int token_of_row(const PromptParams &p, int r) {
+    if (p.gqa_mul == 0) return r;
+    const int q = (int) __umulhi((uint32_t) r, p.gqa_mul);
+    return q * p.gqa > r ? q - 1 : q;
+}
+
 // Inclusive sum over the wave's lanes.
 __device__ __forceinline__ int lane_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
@@ -386,10 +394,7 @@ __global__ __launch_bounds__(NW * 64)
     // ---- the wave's rows: token i of the lane's row, and the tokens it sees, [lo, end) ----
     const int row = row0 + n;
     const bool live = row < rows;
-    // token of row r of the workgroup's: one division for all of them, the rest exact in fp32 (below 2^24)
-    const int base = wg0 / p.gqa, off = wg0 - base * p.gqa;
-    const float inv_gqa = 1.f / (float) p.gqa;
-    auto token_of = [&](int r) { return base + (int) (((float) (r - wg0 + off) + 0.5f) * inv_gqa); };
+    auto token_of = [&](int r) { return token_of_row(p, r); };
     const int i = live ? token_of(row) : 0, head = hk * p.gqa + (live ? row - i * p.gqa : 0);
     const int64_t t = q0 + i;
     int end = 0;
@@ -398,7 +403,7 @@ __global__ __launch_bounds__(NW * 64)
     // of the wave: the tokens that all of its rows see, [w_lo_all, w_end_all), and that any sees, [w_lo, w_end)
     const int i_first = token_of(row0), i_last = token_of(min(row0 + 31, rows - 1));
     // of the workgroup: its tiles start in [g_lo, g_end), and all of its rows see [g_lo_all, g_end_all)
-    const int g_first = base, g_last = token_of(min(wg0 + ROWS, rows) - 1);
+    const int g_first = token_of(wg0), g_last = token_of(min(wg0 + ROWS, rows) - 1);
     int w_end, w_end_all, g_end, g_end_all;
     if (p.row_end) {
         int mx = end, mn = live ? end : INT32_MAX;

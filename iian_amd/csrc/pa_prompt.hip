@@ -13,8 +13,8 @@ hipError_t launch_prompt_f16(const PromptParams &p, hipStream_t stream) {
 }
 
 hipError_t launch_prompt(const PromptParams &p, int type, hipStream_t stream) {
-    // (token numbers within a workgroup come from an fp32 product; millions of tiny prompts would pass a launch's size)
-    if (std::max(p.D, p.Dv) > 256 || p.gqa > 65536 || prompt_blocks(p, 128) > kPromptMaxBlocks)
+    // (millions of tiny prompts would pass a launch's size)
+    if (std::max(p.D, p.Dv) > 256 || prompt_blocks(p, 128) > kPromptMaxBlocks)
         return launch_prompt_rows(p, type, stream);
     switch (type) {
         case 0: return launch_prompt_f32(p, stream);
