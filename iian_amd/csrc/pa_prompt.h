@@ -932,7 +932,13 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
 
 // KW4, KW2: whether waves may share rows by four, by two (LDS holds their tiles).
 // They do in calls whose workgroups then still run at once: one of KW = 4 fits a
-// CU, two of KW = 2.
+// CU, two of KW = 2 (one 512-token prompt, H32/Hkv8/D128 bf16, 13 us, 20 with
+// KW = 1; one of 1024 23 and 33, and 48 with KW = 4).  Long causal prompts share by
+// two up to twice that (three times at head size 64): their last row blocks
+// see the most tokens and are the call's critical path (one of 2048 tokens 53
+// us, 59 with KW = 1, at H20/Hkv20/D96 32 and 46, one of 4096 at H14/Hkv2/D64 48
+// and 74; beyond, KW = 1: one of 2600, D128, 84 and 78; and for short prompts
+// or those that see all: 4 of 512 27 and 22, 2 images of 2048, D80, 73 and 62).
 //
 // NW8: whether the workgroups of the largest calls have 8 waves (head size 256).
 template <int TY, int DK, int DV, bool KW4, bool KW2, bool NW8 = false>
@@ -940,8 +946,12 @@ static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t s
     if (!vec) return launch_prompt_k<TY, DK, DV, false, 1, 4>(p, stream);
     if constexpr (KW4)
         if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4, 4>(p, stream);
-    if constexpr (KW2)
-        if (prompt_blocks(p, 64) <= (KW4 ? 2 : 1) * kPromptCus) return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
+    if constexpr (KW2) {
+        const int64_t at_once = (KW4 ? 2 : 1) * kPromptCus;
+        const bool critical = KW4 && (p.causal || p.row_end) && p.max_q >= 1500;
+        if (prompt_blocks(p, 64) <= at_once * (!critical ? 1 : DK <= 64 ? 3 : 2))
+            return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
+    }
     if constexpr (NW8)
         if (prompt_blocks(p, 256) > kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
     return launch_prompt_k<TY, DK, DV, true, 1, 4>(p, stream);
