@@ -938,9 +938,12 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
 // see the most tokens and are the call's critical path (one of 2048 tokens 53
 // us, 59 with KW = 1, at H20/Hkv20/D96 32 and 46, one of 4096 at H14/Hkv2/D64 48
 // and 74; beyond, KW = 1: one of 2600, D128, 84 and 78; and for short prompts
-// or those that see all: 4 of 512 27 and 22, 2 images of 2048, D80, 73 and 62).
+// or those that see all: 4 of 512 27 and 22, 2 images of 2048, D80, 73 and 62;
+// D256, H16/Hkv8: one of 2048 77 and 89, 4 of 1000 92 and 61).
 //
-// NW8: whether the workgroups of the largest calls have 8 waves (head size 256).
+// NW8: whether workgroups have 8 waves (head size 256) where every CU then still
+// has one (4 prompts of 1000 tokens, H16/Hkv8, 57 us, 61 with 4 waves; 2 images of
+// 2048 123 and 178; below, one causal prompt of 2048 95 and 89).
 template <int TY, int DK, int DV, bool KW4, bool KW2, bool NW8 = false>
 static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
     if (!vec) return launch_prompt_k<TY, DK, DV, false, 1, 4>(p, stream);
@@ -948,12 +951,12 @@ static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t s
         if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4, 4>(p, stream);
     if constexpr (KW2) {
         const int64_t at_once = (KW4 ? 2 : 1) * kPromptCus;
-        const bool critical = KW4 && (p.causal || p.row_end) && p.max_q >= 1500;
+        const bool critical = (p.causal || p.row_end) && p.max_q >= 1500;
         if (prompt_blocks(p, 64) <= at_once * (!critical ? 1 : DK <= 64 ? 3 : 2))
             return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
     }
     if constexpr (NW8)
-        if (prompt_blocks(p, 256) > kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
+        if (prompt_blocks(p, 256) >= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
     return launch_prompt_k<TY, DK, DV, true, 1, 4>(p, stream);
 }
 
