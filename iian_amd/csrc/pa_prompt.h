@@ -89,9 +89,10 @@ struct PromptShape {
     static_assert(PPT * THREADS == TT * CPR, "pieces divide evenly");
     // Q pieces (of KS) that wait in LDS instead of registers: with 8 waves of head size 256, O and half of Q fit the 256
     // registers that two waves per SIMD have
-    static constexpr int QL = NW == 8 ? KS * 5 / 8 : 0;
+    static constexpr int QL = NW == 8 && DK > 128 ? KS * 5 / 8 : 0;
     // waves per SIMD asked of the register allocator
     static constexpr int WAVES = DK > 128 ? NW / 4 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
+    static constexpr int RD = TY == 0 && DK > 128 ? 2 : 3;   // operands held: read RD - 1 products ahead
     __device__ static __forceinline__ int swz(int r) {
         return CPR == 8 ? ((r & 2) << 1) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
     }
@@ -609,22 +610,23 @@ __global__ __launch_bounds__(NW * 64)
 
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     // ---- the tile loop ----
-    // Operands are read two products ahead; the scheduling barriers keep the compiler from pulling each read down to its
+    // Operands are read ahead of their products; the scheduling barriers keep the compiler from pulling each read down to its
     // product, where the wave would wait for it.
     constexpr int NQ = NO * (NS / 8);   // products (triples of them, F32) of a tile with V; KS with K
-    u32x4 kr[3][NP], vr[3][NP], qv[3];
+    constexpr int RD = SH::RD;
+    u32x4 kr[RD][NP], vr[RD][NP], qv[RD];
     auto read_k = [&](int k, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < NP; e++)
-            kr[k % 3][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE);
-        if (k >= QR) qv[k % 3] = ql[(k - QR) * 64];
+            kr[k % RD][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE);
+        if (k >= QR) qv[k % RD] = ql[(k - QR) * 64];
     };
     auto read_v = [&](int q, int buf) __attribute__((always_inline)) {
         const int st = q / NO, m = q % NO;
 #pragma unroll
         for (int e = 0; e < NP; e++) {
             const uint32_t off = buf * SH::BUF + e * SH::PLANE + 16 * st * SH::STRIDE;
-            vr[q % 3][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
+            vr[q % RD][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
         }
     };
     // Tile c0 of the workgroup, in buffer buf_: the wave's part of it begins at cw.
@@ -654,16 +656,16 @@ __global__ __launch_bounds__(NW * 64)
             f32x16 sc;
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[r] = 0.f;
-            read_k(0, buf);
-            read_k(1, buf);
+#pragma unroll
+            for (int k = 0; k < RD - 1; k++) read_k(k, buf);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                if (k + 2 < KS) read_k(k + 2, buf);
-                sc = prompt_mfma<TY>(kr[k % 3][0], k < QR ? qr[0][k < QR ? k : 0] : qv[k % 3], sc);
+                if (k + RD - 1 < KS) read_k(k + RD - 1, buf);
+                sc = prompt_mfma<TY>(kr[k % RD][0], k < QR ? qr[0][k < QR ? k : 0] : qv[k % RD], sc);
                 if constexpr (F32) {
-                    sc = prompt_mfma<TY>(kr[k % 3][NP - 1], qr[0][k], sc);
-                    sc = prompt_mfma<TY>(kr[k % 3][0], qr[NP - 1][k], sc);
+                    sc = prompt_mfma<TY>(kr[k % RD][NP - 1], qr[0][k], sc);
+                    sc = prompt_mfma<TY>(kr[k % RD][0], qr[NP - 1][k], sc);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -754,8 +756,8 @@ __global__ __launch_bounds__(NW * 64)
                 pr[0][st][e] = pack2<TY>(x[8 * st + 2 * e], x[8 * st + 2 * e + 1]);
                 l = sum2<TY>(pr[0][st][e], l);
             };
-            read_v(0, buf);
-            read_v(1, buf);
+#pragma unroll
+            for (int q = 0; q < RD - 1; q++) read_v(q, buf);
             if constexpr (!F32) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) weigh(0, e);
@@ -764,11 +766,11 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
             for (int q = 0; q < NQ; q++) {
                 const int st = q / NO, m = q % NO;
-                if (q + 2 < NQ) read_v(q + 2, buf);
-                o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[0][st], o[m]);
+                if (q + RD - 1 < NQ) read_v(q + RD - 1, buf);
+                o[m] = prompt_mfma<TY>(vr[q % RD][0], pr[0][st], o[m]);
                 if constexpr (F32) {
-                    o[m] = prompt_mfma<TY>(vr[q % 3][NP - 1], pr[0][st], o[m]);
-                    o[m] = prompt_mfma<TY>(vr[q % 3][0], pr[NP - 1][st], o[m]);
+                    o[m] = prompt_mfma<TY>(vr[q % RD][NP - 1], pr[0][st], o[m]);
+                    o[m] = prompt_mfma<TY>(vr[q % RD][0], pr[NP - 1][st], o[m]);
                 } else if (st + 1 < NS / 8) {
 #pragma unroll
                     for (int e = 4 * m / NO; e < 4 * (m + 1) / NO; e++) weigh(st + 1, e);
