@@ -89,7 +89,8 @@ struct PromptShape {
     static_assert(PPT * THREADS == TT * CPR, "pieces divide evenly");
     // Q pieces (of KS) that wait in LDS instead of registers: with 8 waves of head size 256, O and half of Q fit the 256
     // registers that two waves per SIMD have
-    static constexpr int QL = NW == 8 && DK > 128 ? KS * 5 / 8 : 0;
+    // (F32 at 256: of Q's lo terms, as many as LDS has room for)
+    static constexpr int QL = DK <= 128 ? 0 : TY == 0 ? 7 : NW == 8 ? KS * 5 / 8 : 0;
     // waves per SIMD asked of the register allocator
     static constexpr int WAVES = DK > 128 ? NW / 4 : TY == 0 || (KW > 1 && DK > 64) ? 2 : 3;
     static constexpr int RD = TY == 0 && DK > 128 ? 2 : 3;   // operands held: read RD - 1 products ahead
@@ -441,7 +442,7 @@ __global__ __launch_bounds__(NW * 64)
     auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (SH::THREADS / CPR); };
     auto piece_dim = [&](int x, int D) __attribute__((always_inline)) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k), lv0 = lds_addr(lds_v);
-    Piece8<TY> ks[DMA ? 1 : SH::PPT], vs[DMA ? 1 : SH::PPT];
+    Piece8<TY> st[DMA ? 1 : SH::PPT];   // of K or of V, on their way through registers
     // 16-bit rows: byte offsets of a thread's pieces from the tile's first row
     uint32_t kvo[SH::PPT], vvo[SH::PPT];
     if constexpr (DMA) {
@@ -452,34 +453,32 @@ __global__ __launch_bounds__(NW * 64)
         }
     }
     const uint32_t lkw = __builtin_amdgcn_readfirstlane(lk0 + wave * 1024), lvw = __builtin_amdgcn_readfirstlane(lv0 + wave * 1024);
-    // Rows c0 .. of a tile into LDS, or registers; nothing from g_end on.
+    // 16-bit rows c0 .. of a tile into LDS; nothing from g_end on.
     auto load_tile = [&](int c0, int buf) __attribute__((always_inline)) {
         if (c0 >= g_end) return;
-        if constexpr (DMA) {
-            const T *const kt = kb + c0 * p.k_stride, *const vt = vb + c0 * p.v_stride;
-            const uint32_t lk = lkw + buf * SH::BUF, lv = lvw + buf * SH::BUF;
-            if (c0 + TT <= L) {
+        const T *const kt = kb + c0 * p.k_stride, *const vt = vb + c0 * p.v_stride;
+        const uint32_t lk = lkw + buf * SH::BUF, lv = lvw + buf * SH::BUF;
+        if (c0 + TT <= L) {
 #pragma unroll
-                for (int x = 0; x < SH::PPT; x++) {
-                    lds_load16_at(kt, kvo[x], lk, x * SH::THREADS * 16);
-                    lds_load16_at(vt, vvo[x], lv, x * SH::THREADS * 16);
-                }
-            } else {
-#pragma unroll
-                for (int x = 0; x < SH::PPT; x++) {
-                    const uint32_t r = min(piece_row(x), L - 1 - c0);
-                    lds_load16_at(kt, (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2, lk, x * SH::THREADS * 16);
-                    lds_load16_at(vt, (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2, lv, x * SH::THREADS * 16);
-                }
+            for (int x = 0; x < SH::PPT; x++) {
+                lds_load16_at(kt, kvo[x], lk, x * SH::THREADS * 16);
+                lds_load16_at(vt, vvo[x], lv, x * SH::THREADS * 16);
             }
         } else {
 #pragma unroll
             for (int x = 0; x < SH::PPT; x++) {
-                const int64_t j = min(c0 + piece_row(x), L - 1);
-                ks[x] = load_piece<TY, VEC, false>(kb + j * p.k_stride, piece_dim(x, p.D), p.D);
-                vs[x] = load_piece<TY, VEC, false>(vb + j * p.v_stride, piece_dim(x, p.Dv), p.Dv);
+                const uint32_t r = min(piece_row(x), L - 1 - c0);
+                lds_load16_at(kt, (r * (uint32_t) p.k_stride + piece_dim(x, p.D)) * 2, lk, x * SH::THREADS * 16);
+                lds_load16_at(vt, (r * (uint32_t) p.v_stride + piece_dim(x, p.Dv)) * 2, lv, x * SH::THREADS * 16);
             }
         }
+    };
+    // The others through registers, K and V in turn: rows c0 .. of a tile of K or V into st.
+    auto load_rows = [&](const T *base, int64_t stride, int D, int c0) __attribute__((always_inline)) {
+        if (c0 >= g_end) return;
+#pragma unroll
+        for (int x = 0; x < SH::PPT; x++)
+            st[x] = load_piece<TY, VEC, false>(base + (int64_t) min(c0 + piece_row(x), L - 1) * stride, piece_dim(x, D), D);
     };
     // F32: the scale of a row's pieces, which are in CPR neighbouring lanes
     auto row_scale = [&](const Piece8<TY> &x, float *up) __attribute__((always_inline)) {
@@ -507,38 +506,41 @@ __global__ __launch_bounds__(NW * 64)
     };
     // (workgroup-uniform) some row of the workgroup does not see all of the tile
     auto partial = [&](int c0) __attribute__((always_inline)) { return c0 < g_lo_all || c0 + TT > g_end_all; };
-    // Loaded rows into LDS; or the wait for tile c0, behind which `newer` tiles may still be on their way.
-    auto put_tile = [&](int c0, int buf, bool newer) __attribute__((always_inline)) {
-        if constexpr (!DMA) {
-            if (c0 >= g_end) return;
-            bool bad = false;
-            const bool part = partial(c0);
+    // st, rows c0 .. of K or V, into LDS
+    auto put_rows = [&](char *lds_at, float *ups, int c0, bool v) __attribute__((always_inline)) {
+        if (c0 >= g_end) return;
+        const bool part = v && partial(c0);
+        bool bad = false;
 #pragma unroll
-            for (int x = 0; x < SH::PPT; x++) {
-                const int at = buf * SH::BUF + (tid + x * SH::THREADS) * 16, r = piece_row(x);
-                float up = 1.f;
-                if constexpr (F32) up = row_scale(ks[x], &k_up[buf][r]);
-                put_piece(ks[x], lds_k + at, up);
-                if (part) bad |= finite_piece<TY>(vs[x]);
-                if constexpr (F32) up = row_scale(vs[x], &v_up[buf][r]);
-                put_piece(vs[x], lds_v + at, up);
-            }
-            if (bad) bad_v = 1;
-        } else {
-            if (newer) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * SH::PPT) : "memory");
-            else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int x = 0; x < SH::PPT; x++) {
+            float up = 1.f;
+            if (part) bad |= finite_piece<TY>(st[x]);
+            if constexpr (F32) up = row_scale(st[x], &ups[piece_row(x)]);
+            put_piece(st[x], lds_at + (tid + x * SH::THREADS) * 16, up);
         }
+        if (bad) bad_v = 1;
+    };
+    // The wait for a tile behind which `newer` ones may still be on their way.
+    auto wait_tile = [&](bool newer) __attribute__((always_inline)) {
+        if (newer) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(2 * SH::PPT) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
 
     // the first tiles are on their way while Q is loaded
     if (tid == 0) bad_v = 0;
-    if constexpr (!DMA) __syncthreads();
-    load_tile(g_lo, 0);
-    if constexpr (NB == 3) load_tile(g_lo + TT, 1);
+    if constexpr (DMA) {
+        load_tile(g_lo, 0);
+        if constexpr (NB == 3) load_tile(g_lo + TT, 1);
+    } else {
+        __syncthreads();
+        load_rows(kb, p.k_stride, p.D, g_lo);
+        put_rows(lds_k, k_up[0], g_lo, false);
+        load_rows(vb, p.v_stride, p.Dv, g_lo);
+    }
 
     // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
-    constexpr int QL = SH::QL, QR = KS - QL;   // the last QL pieces in LDS
-    u32x4 qr[NP][QR];
+    constexpr int QL = SH::QL, QR = KS - QL;   // the last QL pieces (F32: of the lo terms) in LDS
+    u32x4 qh[F32 ? KS : QR], qlo[F32 ? QR : 1];
     u32x4 *const ql = q_lds + wave * QL * 64 + lane;
     // of the product; above zero, so that a masked score stays -inf (a scale of zero takes Q as zero instead)
     float cs = p.scale == 0.f ? 1.f : fabsf(p.softcap > 0.f ? p.scale / p.softcap : p.scale * kLog2e);
@@ -551,7 +553,7 @@ __global__ __launch_bounds__(NW * 64)
                 u32x4 x = load_piece<TY, VEC, true>(qp, 16 * k + 8 * h, p.D, live).a;
 #pragma unroll
                 for (int e = 0; e < 4; e++) x[e] = p.scale == 0.f ? 0 : x[e] ^ sign;
-                if (k < QR) qr[0][k] = x;
+                if (k < QR) qh[k] = x;
                 else ql[(k - QR) * 64] = x;
             }
         } else {
@@ -566,23 +568,27 @@ __global__ __launch_bounds__(NW * 64)
             const float up = p.scale == 0.f ? 0.f : p.scale < 0.f ? -pow2(15 - ex) : pow2(15 - ex);
             cs *= pow2(ex - 15);
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++) {
+                u32x4 lw;
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const f32x4 &y = e < 2 ? x[k].a : x[k].b;
                     uint32_t a, b;
                     split2(y[2 * (e & 1)] * up, y[2 * (e & 1) + 1] * up, a, b);
-                    qr[0][k][e] = a;
-                    qr[NP - 1][k][e] = b;
+                    qh[k][e] = a;
+                    lw[e] = b;
                 }
+                if (k < QR) qlo[k < QR ? k : 0] = lw;
+                else ql[(k - QR) * 64] = lw;
+            }
         }
         cs = fmaxf(cs, 1e-37f);
         // Q is here: no wait for it (and with it for the tile in flight) inside the loop
 #pragma unroll
-        for (int k = 0; k < QR; k++) {
-            asm volatile("" : "+v"(qr[0][k]));
-            if constexpr (F32) asm volatile("" : "+v"(qr[NP - 1][k]));
-        }
+        for (int k = 0; k < (F32 ? KS : QR); k++) asm volatile("" : "+v"(qh[k]));
+        if constexpr (F32)
+#pragma unroll
+            for (int k = 0; k < QR; k++) asm volatile("" : "+v"(qlo[k]));
     }
 
     f32x16 o[NO];
@@ -629,11 +635,14 @@ __global__ __launch_bounds__(NW * 64)
             vr[q % RD][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
         }
     };
-    // Tile c0 of the workgroup, in buffer buf_: the wave's part of it begins at cw.
+    // Tile c0 of the workgroup, in buffer buf_; the wave's part of it begins at cw.  Into buffer `ahead` another is loaded
+    // meanwhile: the one after next (NB = 3), or the next.
     auto tile = [&](int c0, auto buf_) __attribute__((always_inline)) {
-        constexpr int buf = decltype(buf_)::value, ahead = (buf + NB - 1) % NB;   // ahead: the tile that is loaded meanwhile
-        load_tile(c0 + (NB - 1) * TT, ahead);
-        if constexpr (DMA) {
+        constexpr int buf = decltype(buf_)::value, ahead = (buf + NB - 1) % NB;
+        if constexpr (!DMA) {
+            load_rows(kb, p.k_stride, p.D, c0 + TT);
+        } else {
+            load_tile(c0 + (NB - 1) * TT, ahead);
             if (partial(c0)) {
                 char *const at = lds_v + buf * SH::BUF + tid * 16;
                 bool bad = false;
@@ -651,7 +660,9 @@ __global__ __launch_bounds__(NW * 64)
             }
         }
         const int cw = c0 + KT * kg;
-        if (cw < w_end && cw + KT > w_lo) {   // wave-uniform: some row sees some of it
+        float x[NS], cx = cs, ref;   // x times cx is the score in log2 units, against ref
+        u32x4 pr[NP][NS / 8];
+        auto weights = [&]() __attribute__((always_inline)) {
             // ---- scores ----
             f32x16 sc;
 #pragma unroll
@@ -662,16 +673,14 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 if (k + RD - 1 < KS) read_k(k + RD - 1, buf);
-                sc = prompt_mfma<TY>(kr[k % RD][0], k < QR ? qr[0][k < QR ? k : 0] : qv[k % RD], sc);
+                sc = prompt_mfma<TY>(kr[k % RD][0], F32 || k < QR ? qh[F32 || k < QR ? k : 0] : qv[k % RD], sc);
                 if constexpr (F32) {
-                    sc = prompt_mfma<TY>(kr[k % RD][NP - 1], qr[0][k], sc);
-                    sc = prompt_mfma<TY>(kr[k % RD][0], qr[NP - 1][k], sc);
+                    sc = prompt_mfma<TY>(kr[k % RD][NP - 1], qh[k], sc);
+                    sc = prompt_mfma<TY>(kr[k % RD][0], k < QR ? qlo[k < QR ? k : 0] : qv[k % RD], sc);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
             // ---- softmax ----
-            float x[NS];
-            float cx = cs;   // x times cx is the score in log2 units
 #pragma unroll
             for (int j = 0; j < NS; j++) {
                 x[j] = sc[j];
@@ -707,8 +716,7 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
                     for (int r = 0; r < 16; r++) o[m][r] *= alpha;
             }
-            const float ref = m_ref;
-            u32x4 pr[NP][NS / 8];
+            ref = m_ref;
             if constexpr (F32) {
 #pragma unroll
                 for (int j = 0; j < NS; j++) {
@@ -748,6 +756,8 @@ __global__ __launch_bounds__(NW * 64)
                         pr[NP - 1][st][e] = b;
                     }
             }
+        };
+        auto products = [&]() __attribute__((always_inline)) {
             // ---- O^T += V^T P^T, the next 16 tokens' probabilities beside the products of 16 ----
             // (the sum is of the rounded probabilities, as the products are)
             auto weigh = [&](int st, int e) __attribute__((always_inline)) {   // pair e of the 16 tokens st
@@ -777,11 +787,25 @@ __global__ __launch_bounds__(NW * 64)
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        const bool sees = cw < w_end && cw + KT > w_lo;   // wave-uniform: some row sees some of it
+        if constexpr (DMA) {
+            if (sees) {
+                weights();
+                products();
+            }
+            wait_tile(NB == 3 && c0 + 2 * TT < g_end);
+        } else {
+            if (sees) weights();
+            put_rows(lds_k + ahead * SH::BUF, k_up[ahead], c0 + TT, false);
+            load_rows(vb, p.v_stride, p.Dv, c0 + TT);
+            if (sees) products();
+            put_rows(lds_v + ahead * SH::BUF, v_up[ahead], c0 + TT, true);
         }
-        put_tile(c0 + TT, (buf + 1) % NB, c0 + (NB - 1) * TT < g_end && NB == 3);
         __syncthreads();
     };
-    put_tile(g_lo, 0, NB == 3 && g_lo + TT < g_end);
+    if constexpr (DMA) wait_tile(NB == 3 && g_lo + TT < g_end);
+    else put_rows(lds_v, v_up[0], g_lo, true);
     __syncthreads();
     for (int c0 = g_lo; c0 < g_end; c0 += NB * TT) {
         tile(c0, std::integral_constant<int, 0>());
