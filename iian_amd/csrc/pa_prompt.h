@@ -179,7 +179,7 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_
 __device__ __forceinline__ float piece_max(const Piece8<0> &x) {
     float m = 0.f;
 #pragma unroll
-    for (int e = 0; e < 4; e++) m = fmaxf(m, fmaxf(fabsf(x.a[e]), fabsf(x.b[e])));
+    for (int e = 0; e < 4; e++) m = fmaxf(fmaxf(m, fabsf(x.a[e])), fabsf(x.b[e]));   // (one instruction each)
     return m;
 }
 template <int CPR>
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(NW * 64)
     auto piece_row = [&](int x) __attribute__((always_inline)) { return pr0 + x * (SH::THREADS / CPR); };
     auto piece_dim = [&](int x, int D) __attribute__((always_inline)) { return min(((tid % CPR) ^ SH::swz(piece_row(x))) * 8, (D - 1) & ~7); };
     const uint32_t lk0 = lds_addr(lds_k), lv0 = lds_addr(lds_v);
-    Piece8<TY> st[DMA ? 1 : SH::PPT];   // of K or of V, on their way through registers
+    Piece8<TY> st[DMA ? 1 : SH::PPT], st0[DMA ? 1 : SH::PPT];   // of K or of V, on their way through registers (st0: the first K)
     // 16-bit rows: byte offsets of a thread's pieces from the tile's first row
     uint32_t kvo[SH::PPT], vvo[SH::PPT];
     if constexpr (DMA) {
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(NW * 64)
         }
     };
     // The others through registers, K and V in turn: rows c0 .. of a tile of K or V into st.
-    auto load_rows = [&](const T *base, int64_t stride, int D, int c0) __attribute__((always_inline)) {
+    auto load_rows = [&](auto &st, const T *base, int64_t stride, int D, int c0) __attribute__((always_inline)) {
         if (c0 >= g_end) return;
 #pragma unroll
         for (int x = 0; x < SH::PPT; x++)
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(NW * 64)
     // (workgroup-uniform) some row of the workgroup does not see all of the tile
     auto partial = [&](int c0) __attribute__((always_inline)) { return c0 < g_lo_all || c0 + TT > g_end_all; };
     // st, rows c0 .. of K or V, into LDS
-    auto put_rows = [&](char *lds_at, float *ups, int c0, bool v) __attribute__((always_inline)) {
+    auto put_rows = [&](auto &st, char *lds_at, float *ups, int c0, bool v) __attribute__((always_inline)) {
         if (c0 >= g_end) return;
         const bool part = v && partial(c0);
         bool bad = false;
@@ -533,9 +533,8 @@ __global__ __launch_bounds__(NW * 64)
         if constexpr (NB == 3) load_tile(g_lo + TT, 1);
     } else {
         __syncthreads();
-        load_rows(kb, p.k_stride, p.D, g_lo);
-        put_rows(lds_k, k_up[0], g_lo, false);
-        load_rows(vb, p.v_stride, p.Dv, g_lo);
+        load_rows(st0, kb, p.k_stride, p.D, g_lo);
+        load_rows(st, vb, p.v_stride, p.Dv, g_lo);
     }
 
     // ---- Q: dims 16 ks + 8h .. + 7 of the lane's row (negated for a negative scale) ----
@@ -597,7 +596,7 @@ __global__ __launch_bounds__(NW * 64)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[m][r] = 0.f;
     float m_ref = -0x1p127f, l = 0.f;   // reference maximum (log2 units, below any score) and the lane's part of the sum
-    float v_ref = 0x1p-126f;            // F32: power of two that V's factors are taken relative to
+    float v_ref = 0x1p-126f, v_inv = 0x1p126f;   // F32: power of two that V's factors are taken relative to, and one over it
 
     // lane's LDS byte offsets.  K row n (+ 32 hh), piece 2k + h; V transpose reads: rows 4h + (lane%16)/4 (+ 8, + 16 st),
     // dims 32m + 16((lane/16)%2) + 4(lane%4): piece 4m + 2((lane/16)%2) + (lane%4)/2, 8 bytes into it for odd lanes.  The
@@ -640,7 +639,7 @@ __global__ __launch_bounds__(NW * 64)
     auto tile = [&](int c0, auto buf_) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_)::value, ahead = (buf + NB - 1) % NB;
         if constexpr (!DMA) {
-            load_rows(kb, p.k_stride, p.D, c0 + TT);
+            load_rows(st, kb, p.k_stride, p.D, c0 + TT);
         } else {
             load_tile(c0 + (NB - 1) * TT, ahead);
             if (partial(c0)) {
@@ -736,14 +735,14 @@ __global__ __launch_bounds__(NW * 64)
                     for (int j = 0; j < NS; j++) top = fmaxf(top, x[j] != 0.f ? vf[j] : 0.f);
                     top = max_halves(top);
                     const float vn = top > v_ref * 64.f ? top : v_ref;
-                    const float beta = v_ref / vn;
+                    const float beta = v_ref * (1.f / vn);   // (powers of two)
                     v_ref = vn;
+                    v_inv = 1.f / vn;
 #pragma unroll
                     for (int m = 0; m < NO; m++)
 #pragma unroll
                         for (int r = 0; r < 16; r++) o[m][r] *= beta;
                 }
-                const float inv = 1.f / v_ref;   // a power of two
 #pragma unroll
                 for (int st = 0; st < NS / 8; st++)
 #pragma unroll
@@ -751,7 +750,7 @@ __global__ __launch_bounds__(NW * 64)
                         // (a token of no weight may have any factor: kept finite)
                         const int j = 8 * st + 2 * e;
                         uint32_t a, b;
-                        split2(x[j] * fminf(vf[j] * inv, 0x1p100f), x[j + 1] * fminf(vf[j + 1] * inv, 0x1p100f), a, b);
+                        split2(x[j] * fminf(vf[j] * v_inv, 0x1p100f), x[j + 1] * fminf(vf[j + 1] * v_inv, 0x1p100f), a, b);
                         pr[0][st][e] = a;
                         pr[NP - 1][st][e] = b;
                     }
@@ -797,15 +796,19 @@ __global__ __launch_bounds__(NW * 64)
             wait_tile(NB == 3 && c0 + 2 * TT < g_end);
         } else {
             if (sees) weights();
-            put_rows(lds_k + ahead * SH::BUF, k_up[ahead], c0 + TT, false);
-            load_rows(vb, p.v_stride, p.Dv, c0 + TT);
+            put_rows(st, lds_k + ahead * SH::BUF, k_up[ahead], c0 + TT, false);
+            load_rows(st, vb, p.v_stride, p.Dv, c0 + TT);
             if (sees) products();
-            put_rows(lds_v + ahead * SH::BUF, v_up[ahead], c0 + TT, true);
+            put_rows(st, lds_v + ahead * SH::BUF, v_up[ahead], c0 + TT, true);
         }
         __syncthreads();
     };
-    if constexpr (DMA) wait_tile(NB == 3 && g_lo + TT < g_end);
-    else put_rows(lds_v, v_up[0], g_lo, true);
+    if constexpr (DMA) {
+        wait_tile(NB == 3 && g_lo + TT < g_end);
+    } else {
+        put_rows(st0, lds_k, k_up[0], g_lo, false);
+        put_rows(st, lds_v, v_up[0], g_lo, true);
+    }
     __syncthreads();
     for (int c0 = g_lo; c0 < g_end; c0 += NB * TT) {
         tile(c0, std::integral_constant<int, 0>());
