@@ -604,13 +604,15 @@ __global__ __launch_bounds__(NW * 64)
     // r + 8 (r + 16 is r again) are V's.
     const int vrow = 4 * h + ((lane & 15) >> 2), vpiece = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
     // (opaque: kept as they are, so that what is added below is a constant of the read)
-    uint32_t koff[KS], voff[2][NO];
+    // (the exclusive or stays within 16 pieces, 256 bytes: past them the patterns come again)
+    constexpr int KP = KS < 8 ? KS : 8, VP = NO < 4 ? NO : 4;
+    uint32_t koff[KP], voff[2][VP];
 #pragma unroll
-    for (int k = 0; k < KS; k++) koff[k] = opaque(lk0 + (KT * kg + n) * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n)));
+    for (int k = 0; k < KP; k++) koff[k] = opaque(lk0 + (KT * kg + n) * SH::STRIDE + 16 * ((2 * k + h) ^ SH::swz(n)));
 #pragma unroll
     for (int e = 0; e < 2; e++)
 #pragma unroll
-        for (int m = 0; m < NO; m++)
+        for (int m = 0; m < VP; m++)
             voff[e][m] = opaque(lv0 + (KT * kg + vrow + 8 * e) * SH::STRIDE + 16 * ((4 * m + vpiece) ^ SH::swz(vrow + 8 * e)) + 8 * (lane & 1));
 
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
@@ -623,15 +625,15 @@ __global__ __launch_bounds__(NW * 64)
     auto read_k = [&](int k, int buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < NP; e++)
-            kr[k % RD][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k] + buf * SH::BUF + e * SH::PLANE);
+            kr[k % RD][e] = *(const lds_u32x4 *) (uintptr_t) (koff[k % KP] + k / KP * 256 + buf * SH::BUF + e * SH::PLANE);
         if (k >= QR) qv[k % RD] = ql[(k - QR) * 64];
     };
     auto read_v = [&](int q, int buf) __attribute__((always_inline)) {
         const int st = q / NO, m = q % NO;
 #pragma unroll
         for (int e = 0; e < NP; e++) {
-            const uint32_t off = buf * SH::BUF + e * SH::PLANE + 16 * st * SH::STRIDE;
-            vr[q % RD][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m] + off, voff[1][m] + off));
+            const uint32_t off = buf * SH::BUF + e * SH::PLANE + 16 * st * SH::STRIDE + m / VP * 256;
+            vr[q % RD][e] = __builtin_bit_cast(u32x4, lds_tr_b16x8_at(voff[0][m % VP] + off, voff[1][m % VP] + off));
         }
     };
     // Tile c0 of the workgroup, in buffer buf_; the wave's part of it begins at cw.  Into buffer `ahead` another is loaded
