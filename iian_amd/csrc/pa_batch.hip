@@ -115,22 +115,29 @@ __global__ __launch_bounds__(256) void pa_swa_free_kernel(const int32_t *__restr
 //
 // Workgroup (s, c) takes the c-th share of request s' new tokens.  It needs the
 // token and position prefix sums over the request's runs up to them: kRunsPer
-// runs per thread, loaded together and summed, a wave scan over the threads and
-// one over the waves, so a round covers 2048 runs and a request of 2000 takes
-// one.  The prefixes go to LDS, where each of the share's tokens finds its run
-// by a binary search.  Every share scans for itself: a request's runs are a few
-// KB and stay in L2, while a scan in a launch of its own would cost the launch.
-// Latency-bound: query_start_loc and span_off, then the runs, then the store.
+// runs per thread, loaded together and summed, a scan over the wave's lanes by
+// lane permutes and one over the waves, so a round covers 2048 runs and a request of
+// 2000 takes one.  The prefixes and the runs go to LDS, where each of the share's
+// tokens finds its run by a binary search.  Every share scans for itself: a
+// request's runs are a few KB and stay in L2, while a scan in a launch of its
+// own would cost the launch.  Sums are held at INT32_MAX (adding and holding is
+// associative), so 32 bits suffice.  Latency-bound: query_start_loc and
+// span_off, then the runs, the search, the stores (kernel trace: 48 decoding
+// requests of 12 runs 4.6 us, 131,072 tokens of 4 requests of 2000 runs 9.0; with
+// 64-bit sums and the run read again from memory 6.4 and 10.1).
 constexpr int kRunsPer = 8;
 constexpr int kRunsRound = 256 * kRunsPer;
+constexpr uint32_t kMost = INT32_MAX;
 
 struct RunExtent {
-    int64_t tokens, advance;
+    uint32_t tokens, advance;   // at most kMost
     bool bad;
 };
 
-// Tokens and position advance of a run, each below 2^31 (a larger one is held
-// at INT32_MAX: prefix sums of 2^31 runs stay within 64 bits).
+__device__ __forceinline__ uint32_t hold(uint64_t v) { return (uint32_t) min(v, (uint64_t) kMost); }
+__device__ __forceinline__ uint32_t sum_held(uint32_t a, uint32_t b) { return min(a + b, kMost); }   // (both at most kMost)
+
+// Tokens and position advance of a run.
 __device__ __forceinline__ RunExtent run_extent(const int4 &r) {
     RunExtent e = {0, 0, false};
     const bool grid = r.y != 0 || r.z != 0;
@@ -139,46 +146,58 @@ __device__ __forceinline__ RunExtent run_extent(const int4 &r) {
     } else if (!grid) {
         e.tokens = e.advance = r.x;
     } else if (r.x > 0) {
-        const int64_t plane = min((int64_t) r.y * r.z, (int64_t) INT32_MAX);
-        e.tokens = min(r.x * plane, (int64_t) INT32_MAX);
-        const int64_t time = (int64_t) (r.x - 1) * max(r.w, 1) + 1;
-        e.advance = min(max(time, (int64_t) max(r.y, r.z)), (int64_t) INT32_MAX);
-        e.bad = r.w < 1 || r.x * plane > INT32_MAX || time > INT32_MAX;
+        const uint64_t tokens = (uint64_t) r.x * hold((uint64_t) (uint32_t) r.y * (uint32_t) r.z);
+        const uint64_t time = (uint64_t) (r.x - 1) * (uint32_t) max(r.w, 1) + 1;
+        e.tokens = hold(tokens);
+        e.advance = max(hold(time), (uint32_t) max(r.y, r.z));
+        e.bad = r.w < 1 || tokens > kMost || time > kMost;
     }
     return e;
 }
 
+// Inclusive held sums over the wave's lanes.
+__device__ __forceinline__ uint32_t scan_held(uint32_t v) {
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));    // row_shr 1, 2, 4, 8
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));   // row_bcast 15 into rows 1 and 3
+    v = sum_held(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));   // row_bcast 31 into rows 2 and 3
+    return v;
+}
+
 __global__ __launch_bounds__(256) void pa_mrope_positions_kernel(MropePosParams p) {
-    __shared__ int64_t wave_sum[2][4];
-    // tokens and position before each run of the round, and after the last
-    __shared__ int32_t tok[kRunsRound + 1], at[kRunsRound + 1];
+    __shared__ uint32_t wave_sum[2][4];
+    // of the round's runs: tokens before each, and behind the last; position before it, h, w (0 for text) and step
+    __shared__ uint32_t tok[kRunsRound + 1];
+    __shared__ __attribute__((aligned(16))) int4 info[kRunsRound];
     const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int f0 = p.span_off[s], f1 = p.span_off[s + 1];
+    const int nc = p.num_computed[s];
     const int q0 = min(max(p.qsl[s], 0), p.T), q1 = min(max(p.qsl[s + 1], q0), p.T);
     const int nn = q1 - q0;
     // shares of whole waves
     const int64_t per = ((int64_t) nn + gridDim.y - 1) / gridDim.y + 63 & ~(int64_t) 63;
     const int i0 = (int) min(blockIdx.y * per, (int64_t) nn), i1 = (int) min(i0 + per, (int64_t) nn);
-    const int f0 = p.span_off[s], f1 = p.span_off[s + 1];
-    const int nc = p.num_computed[s];
     const int b0 = min(max(f0, 0), p.n_spans), b1 = min(max(f1, b0), p.n_spans);
     bool bad = nc < 0 || f0 != b0 || f1 != b1;
-    const bool first = blockIdx.y == 0;   // flags each request once, whether it has new tokens or not
-    if (i0 >= i1 && !first) return;
-    const int64_t r0 = (int64_t) max(nc, 0) + i0, r1 = (int64_t) max(nc, 0) + i1;   // the share's tokens of the request
-    int64_t tok0 = 0, at0 = 0;   // before the round
-    int64_t done = r0;           // tokens written so far
-    auto put = [&](int64_t r, int64_t pt, int64_t ph, int64_t pw, int64_t end) {
+    if (i0 >= i1 && blockIdx.y != 0) return;   // (the first share flags a request, whether it has new tokens or not)
+    const uint32_t r0 = (uint32_t) max(nc, 0) + i0, r1 = (uint32_t) max(nc, 0) + i1;   // the share's tokens of the request
+    uint32_t tok0 = 0, at0 = 0;   // before the round
+    uint32_t done = r0;           // tokens written so far
+    auto put = [&](uint32_t r, uint64_t pt, uint64_t ph, uint64_t pw, uint64_t end) {
         const int t = q0 + (int) (r - max(nc, 0));
-        bad |= pt > INT32_MAX || ph > INT32_MAX || pw > INT32_MAX || end > INT32_MAX;
-        p.pos[t] = (int32_t) min(pt, (int64_t) INT32_MAX);
-        p.pos[(int64_t) p.T + t] = (int32_t) min(ph, (int64_t) INT32_MAX);
-        p.pos[2 * (int64_t) p.T + t] = (int32_t) min(pw, (int64_t) INT32_MAX);
-        if (p.row_end) p.row_end[t] = (int32_t) min(end, (int64_t) INT32_MAX);
+        bad |= max(max(pt, ph), max(pw, end)) > kMost;
+        p.pos[t] = (int32_t) hold(pt);
+        p.pos[(int64_t) p.T + t] = (int32_t) hold(ph);
+        p.pos[2 * (int64_t) p.T + t] = (int32_t) hold(pw);
+        if (p.row_end) p.row_end[t] = (int32_t) hold(end);
     };
     for (int b = b0; b < b1 && done < r1; b += kRunsRound) {
         const int n = min(kRunsRound, b1 - b);
         int4 run[kRunsPer];
-        int64_t ts = 0, as = 0;
+        RunExtent e[kRunsPer];
+        uint32_t ts = 0, as = 0;
 #pragma unroll
         for (int k = 0; k < kRunsPer; k++) {
             const int j = tid * kRunsPer + k;
@@ -186,74 +205,71 @@ __global__ __launch_bounds__(256) void pa_mrope_positions_kernel(MropePosParams 
         }
 #pragma unroll
         for (int k = 0; k < kRunsPer; k++) {
-            const RunExtent e = run_extent(run[k]);
-            bad |= e.bad;
-            ts += e.tokens;
-            as += e.advance;
+            e[k] = run_extent(run[k]);
+            bad |= e[k].bad;
+            ts = sum_held(ts, e[k].tokens);
+            as = sum_held(as, e[k].advance);
         }
-        int64_t tp = ts, ap = as;   // inclusive scans over the wave's lanes
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int64_t x = __shfl_up(tp, o), y = __shfl_up(ap, o);
-            if (lane >= o) {
-                tp += x;
-                ap += y;
-            }
-        }
+        const uint32_t tp = scan_held(ts), ap = scan_held(as);
         if (lane == 63) {
             wave_sum[0][wave] = tp;
             wave_sum[1][wave] = ap;
         }
+        // (held sums do not subtract: what is before the lane is the lane's below)
+        uint32_t tw = __shfl_up(tp, 1), aw = __shfl_up(ap, 1);
+        if (lane == 0) tw = aw = 0;
         __syncthreads();
-        int64_t tw = tok0, aw = at0;
+        uint32_t tb = tok0, ab = at0;
+#pragma unroll
         for (int w = 0; w < 4; w++) {
             if (w < wave) {
-                tw += wave_sum[0][w];
-                aw += wave_sum[1][w];
+                tb = sum_held(tb, wave_sum[0][w]);
+                ab = sum_held(ab, wave_sum[1][w]);
             }
-            tok0 += wave_sum[0][w];
-            at0 += wave_sum[1][w];
+            tok0 = sum_held(tok0, wave_sum[0][w]);
+            at0 = sum_held(at0, wave_sum[1][w]);
         }
-        tw += tp - ts;
-        aw += ap - as;
+        tw = sum_held(tw, tb);
+        aw = sum_held(aw, ab);
+        if (tid * kRunsPer < n) {
 #pragma unroll
-        for (int k = 0; k < kRunsPer; k++) {
-            tok[tid * kRunsPer + k] = (int32_t) min(tw, (int64_t) INT32_MAX);
-            at[tid * kRunsPer + k] = (int32_t) min(aw, (int64_t) INT32_MAX);
-            const RunExtent e = run_extent(run[k]);
-            tw += e.tokens;
-            aw += e.advance;
+            for (int k = 0; k < kRunsPer; k++) {
+                tok[tid * kRunsPer + k] = tw;
+                info[tid * kRunsPer + k] = make_int4((int) aw, run[k].y, run[k].y > 0 ? run[k].z : 0, max(run[k].w, 1));
+                tw = sum_held(tw, e[k].tokens);
+                aw = sum_held(aw, e[k].advance);
+            }
         }
-        if (tid == 255) {
-            tok[kRunsRound] = (int32_t) min(tw, (int64_t) INT32_MAX);
-            at[kRunsRound] = (int32_t) min(aw, (int64_t) INT32_MAX);
-        }
+        if (tid == 0) tok[n] = tok0;
         __syncthreads();
-        const int64_t stop = min(r1, tok0);   // the round's runs hold tokens up to tok0
-        for (int64_t r = done + tid; r < stop; r += 256) {
+        const uint32_t stop = min(r1, tok0);   // the round's runs hold tokens up to tok0
+        for (uint32_t r = done + tid; r < stop; r += 256) {
             // the last run that starts at or before token r: it holds r, since the
             // runs of no tokens behind it start where the next one does
-            int lo = 0, hi = kRunsRound;
+            int lo = 0, hi = n;
             while (hi - lo > 1) {
                 const int m = (lo + hi) >> 1;
                 if (tok[m] <= r) lo = m;
                 else hi = m;
             }
-            const int4 g = p.spans[b + min(lo, n - 1)];
-            const uint32_t i = (uint32_t) (r - tok[lo]);
-            const int64_t base = at[lo];
-            if (g.y > 0 && g.z > 0) {
+            const int4 g = info[lo];
+            const uint32_t i = r - tok[lo];
+            const uint64_t base = (uint32_t) g.x;
+            if (g.z > 0) {
                 const uint32_t w = (uint32_t) g.z, h = (uint32_t) g.y, row = i / w, it = row / h;
-                put(r, base + (int64_t) it * max(g.w, 1), base + (row - it * h), base + (i - row * w),
-                    p.grid_full ? (int64_t) tok[lo + 1] : r + 1);
+                put(r, base + (uint64_t) it * (uint32_t) g.w, base + (row - it * h), base + (i - row * w),
+                    p.grid_full ? (uint64_t) tok[lo + 1] : (uint64_t) r + 1);
             } else {
-                put(r, base + i, base + i, base + i, r + 1);
+                put(r, base + i, base + i, base + i, (uint64_t) r + 1);
             }
         }
         done = max(done, stop);
         __syncthreads();   // the prefixes are rewritten by the next round
     }
-    for (int64_t r = done + tid; r < r1; r += 256) put(r, at0 + (r - tok0), at0 + (r - tok0), at0 + (r - tok0), r + 1);
+    for (uint32_t r = done + tid; r < r1; r += 256) {
+        const uint64_t at = (uint64_t) at0 + (r - tok0);
+        put(r, at, at, at, (uint64_t) r + 1);
+    }
     if (bad && p.err) atomicOr(p.err, 8);
 }
 
