@@ -40,13 +40,13 @@ __device__ __forceinline__ float mrope_f32(float x) { return x; }
 __device__ __forceinline__ float mrope_f32(_Float16 x) { return (float) x; }
 __device__ __forceinline__ float mrope_f32(bf16_t x) { return (float) x; }
 
-// (cos, sin) of pos * freq, times mscale.
+// (cos, sin) of pos * freq, times mscale.  (The fraction is of |freq|: that of a tiny negative one would round to a whole turn.)
 __device__ __forceinline__ float2 mrope_cs(double freq, int pos, float mscale) {
-    const double turns = freq * 0.15915494309189533576888;   // 1 / (2 pi)
+    const double turns = fabs(freq) * 0.15915494309189533576888;   // 1 / (2 pi)
     const double fr = turns - floor(turns);
     const double up = fr * 4294967296.0, hi = floor(up);
     const uint64_t step = ((uint64_t) (uint32_t) hi << 32) | (uint32_t) ((up - hi) * 4294967296.0);
-    const uint64_t u = step * (uint64_t) (int64_t) pos;
+    const uint64_t u = step * (uint64_t) (freq < 0 ? -(int64_t) pos : (int64_t) pos);
     const uint32_t quad = (uint32_t) ((u + (1ull << 61)) >> 62);
     const int32_t rest = (int32_t) ((u - ((uint64_t) quad << 62)) >> 32);   // [-2^29, 2^29) of 2^32 a turn
     const float x = (float) rest * 1.46291807926715968e-9f;                 // 2 pi 2^-32: [-pi/4, pi/4)

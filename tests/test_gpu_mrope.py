@@ -305,6 +305,26 @@ def test_an_axis_outside_is_held_inside(pa):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 66])
+def test_negative_frequencies_turn_back(pa, D):
+    """Rotated by a table and then by its negative, a row is itself again; tiny frequencies of either sign turn nothing."""
+    T = 50
+    k = torch.randn(T, 2, D, device="cuda")
+    pos = torch.randint(-4000, 1000000, (1, T), dtype=torch.int32, device="cuda")
+    fr = 1e4 ** (-torch.arange(D // 2, dtype=torch.float64, device="cuda") / (D // 2))
+    ax = torch.zeros(D // 2, dtype=torch.int32, device="cuda")
+    a, b = torch.empty_like(k), torch.empty_like(k)
+    pa.mrope_set_rows_kv(None, None, k, None, None, pos, fr, ax, k_out=a)
+    pa.mrope_set_rows_kv(None, None, a, None, None, pos, -fr, ax, k_out=b)
+    pair = (k[..., :D // 2] ** 2 + k[..., D // 2:] ** 2).sqrt().repeat(1, 1, 2)
+    assert ((b - k).abs() <= 2.8e-6 * pair).all()
+    pos.fill_(2147483647)
+    for tiny in (1e-18, -1e-18, -1e-300):
+        pa.mrope_set_rows_kv(None, None, k, None, None, pos, 0 * fr + tiny, ax, k_out=a)
+        assert ((a - k).abs() <= 1.4e-6 * pair).all()
+
+
+@pytest.mark.gpu
 def test_one_axis_agrees_with_the_rope_write(pa):
     """All axes at the token's index: the rotation iian_pa_rope_kv_write makes, whose chained fp32 angle is off by
     up to (j + 1) roundings of 2^-24 at pair j: at position p < 64, 64 * p * 2^-24 < 2.5e-4 of the pair."""
