@@ -59,7 +59,9 @@ constexpr int kMaxWavesPerCu = kQ8DecodeWavesPerCu;
 constexpr int kDefaultCus = 256;   // an MI355X, when the device cannot be queried
 constexpr int kMaxHeadDim = 1024;  // largest head size the general kernel stages (pa_general.hip)
 constexpr int kMaxSeqs = 1 << 23;             // of the multi-axis positions and whole-prompt attention: a workgroup each stays within a launch's 2^32 threads
-constexpr int kMaxPromptTokens = 1 << 30;   // iian_pa_prompt_attention counts tokens and tiles past them in 32 bits
+constexpr int kMaxPromptTokens = 1 << 30;   // iian_pa_prompt_attention counts tokens and tiles past them in 32 bits,
+constexpr int kMaxPromptRows = INT32_MAX - 1024;   // and a prompt's rows with a workgroup's beyond
+constexpr int kMaxSpans = 1 << 30;          // runs of iian_pa_mrope_positions, which steps past the last by up to 2048
 constexpr int kMaxDevices = 64;
 
 // Compute units of device `dev`, queried once per device.
@@ -898,7 +900,8 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
 int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
                             const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
                             int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag) {
-    if (n_seqs < 0 || n_seqs > kMaxSeqs || n_tokens < 0 || n_spans < 0) return IIAN_PA_ERR_ARG;
+    if (n_seqs < 0 || n_seqs > kMaxSeqs || n_tokens < 0 || n_spans < 0 || n_spans > kMaxSpans)
+        return IIAN_PA_ERR_ARG;
     if (n_seqs == 0 || n_tokens == 0) return IIAN_PA_OK;
     if ((n_spans > 0 && !spans) || !span_off || !num_computed || !query_start_loc || !pos) return IIAN_PA_ERR_NULL;
     if ((uintptr_t) spans & 15) return IIAN_PA_ERR_ARG;   // a run is one 16-byte load
@@ -1073,7 +1076,7 @@ int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const v
     if (n_swa < 0 || softcap < 0.0f || !std::isfinite(scale) || !std::isfinite(softcap)) return IIAN_PA_ERR_ARG;
     const int esize = row_type_bytes(type);
     if (!esize || head_dim > kMaxHeadDim || head_dim_v > kMaxHeadDim) return IIAN_PA_ERR_UNSUPPORTED;
-    if ((int64_t) n_head * std::max(head_dim, head_dim_v) > INT32_MAX / 2 || (int64_t) n_tokens * n_head > INT32_MAX)
+    if ((int64_t) n_head * std::max(head_dim, head_dim_v) > INT32_MAX / 2 || (int64_t) n_tokens * n_head > kMaxPromptRows)
         return IIAN_PA_ERR_ARG;
     if (q_stride < (int64_t) n_head * head_dim || k_stride < (int64_t) n_head_kv * head_dim ||
         v_stride < (int64_t) n_head_kv * head_dim_v || out_stride < (int64_t) n_head * head_dim_v)

@@ -326,7 +326,7 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
  * with h or w zero or a step below 1 (its tokens then count as none, its step
  * as 1), offsets out of order or outside [0, n_spans], or a position or end
  * past INT32_MAX, which is held there; seen in the runs that the step's tokens
- * need, those up to them.  At most 2^23 requests. */
+ * need, those up to them.  At most 2^23 requests and 2^30 runs. */
 int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
                             const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
                             int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag);
@@ -384,7 +384,7 @@ typedef struct {
  * positions are as precise as near ones.  mode is rope's: 0 pairs (2j, 2j+1),
  * 2 pairs (j, j + n_dims/2); values past n_dims are copied (normed, not scaled).
  *   pos    int32 [n_axes][n_rows]; any value, negative ones included
- *   freqs  double [n_dims/2], axis int32 [n_dims/2] (device; an axis outside
+ *   freqs  double [n_dims/2], finite (a negative one turns back), axis int32 [n_dims/2] (device; an axis outside
  *          [0, n_axes) is taken as the nearest one inside)
  * The pools, their types, slots and *err_flag bit 0 are iian_pa_kv_write's;
  * k_pool, v_pool and slots may all be NULL when k_out is given (a vision
@@ -413,12 +413,12 @@ int iian_pa_mrope_kv_write(void *stream, const iian_pa_mrope_rows *rows, const i
  *   q [T][n_head][head_dim], k [T][n_head_kv][head_dim], v [T][n_head_kv][head_dim_v],
  *   out [T][n_head][head_dim_v], all of `type` (F32, F16 or BF16), tokens of
  *   q, k, v and out *_stride elements apart; aligned to their element
- *   max_query_len  host int: the longest prompt's tokens (or more); rows of a
+ *   max_query_len  host int, 1 to n_tokens: the longest prompt's tokens (or more); rows of a
  *                  longer one past it may be left unwritten and set bit 2 of *err_flag
  * Scores, sums and softmax statistics are fp32; F16 and BF16 rows enter the
  * matrix products as they are and probabilities rounded to their type, F32
  * rows as pairs of f16 terms (22 bits).  Head sizes 1 to 1024, at most 2^23
- * prompts, n_tokens * n_head below 2^31.  No workspace. */
+ * prompts, 2^30 tokens, n_tokens * n_head at most 2^31 - 1025.  No workspace. */
 int iian_pa_prompt_attention(void *stream, const void *q, const void *k, const void *v, int type, int64_t q_stride,
                              int64_t k_stride, int64_t v_stride, const int32_t *query_start_loc,
                              const int32_t *row_end, int32_t n_tokens, int32_t n_seqs, int32_t max_query_len,

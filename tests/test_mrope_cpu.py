@@ -82,7 +82,7 @@ def positions(**over):
 
 @pytest.mark.parametrize("over,code", [
     ({"spans": None}, -1), ({"off": None}, -1), ({"nc": None}, -1), ({"qsl": None}, -1), ({"pos": None}, -1),
-    ({"S": -1}, -2), ({"T": -1}, -2), ({"n_spans": -1}, -2), ({"spans": 0x1008}, -2), ({"S": 0}, 0), ({"T": 0}, 0),
+    ({"S": -1}, -2), ({"T": -1}, -2), ({"n_spans": -1}, -2), ({"n_spans": 2 ** 31 - 1}, -2), ({"spans": 0x1008}, -2), ({"S": 0}, 0), ({"T": 0}, 0),
 ])
 def test_positions_refused(over, code):
     assert positions(**over) == code
@@ -135,7 +135,8 @@ def prompt(**over):
     ({"scale": math.nan}, -2), ({"cap": math.inf}, -2), ({"type": 8}, -3), ({"type": 2}, -3),
     ({"D": 1025, "qs": 9000, "ks": 9000}, -3), ({"qs": 1023}, -2), ({"ks": 255}, -2), ({"vs": 255}, -2),
     ({"os": 1023}, -2), ({"q": 0x10001}, -2), ({"out": 0x50001}, -2), ({"type": 0, "v": 0x30002}, -2),
-    ({"end": 0x60002}, -2), ({"T": 1 << 30, "maxq": 1}, -2), ({"T": 0}, 0), ({"S": 0}, 0),
+    ({"end": 0x60002}, -2), ({"T": 1 << 30, "maxq": 1}, -2), ({"T": (1 << 31) - 1, "H": 1, "Hkv": 1, "maxq": 1}, -2),
+    ({"T": (1 << 30) - 1, "H": 2, "Hkv": 1, "maxq": 1}, -2), ({"T": 0}, 0), ({"S": 0}, 0),
 ])
 def test_prompt_refused(over, code):
     assert prompt(**over) == code
