@@ -400,6 +400,7 @@ __global__ __launch_bounds__(NW * 64)
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, h = lane >> 5;
     if (blk.rb == 0 && hk == 0 && tid == 0 && L > p.max_q && p.err) atomicOr(p.err, 4);
     const int rows = min(L, p.max_q) * p.gqa;   // (the host holds tokens times heads below 2^31)
+    if ((uint32_t) blk.rb > (uint32_t) rows / ROWS) return;   // (counts of an out-of-order query_start_loc may pass 32 bits)
     const int wg0 = blk.rb * ROWS, row0 = wg0 + 32 * (wave / KW), kg = wave % KW;
 
     // ---- the wave's rows: token i of the lane's row, and the tokens it sees, [lo, end) ----

@@ -174,6 +174,41 @@ def test_many_prompts_masked(pa, kw, kind):
     one(pa, MANY, 16, 8, 128, kind=kind, ends=ends, **{k: v for k, v in kw.items() if k not in ("images", "empty")})
 
 
+@pytest.mark.parametrize("D,kind", [(64, "f16"), (80, "bf16"), (96, "f32"), (256, "bf16"), (256, "f32")])
+@pytest.mark.parametrize("kw", [dict(causal=False), dict(n_swa=50, softcap=8.0), dict(images=True, n_swa=90), dict(empty=True)], ids=str)
+def test_many_prompts_masked_at_other_head_sizes(pa, D, kind, kw):
+    ends = image_ends if kw.get("images") else ENDS["any"] if kw.get("empty") else None
+    one(pa, MANY, 16, 8, D, kind=kind, ends=ends, lead=1, **{k: v for k, v in kw.items() if k not in ("images", "empty")})
+
+
+@pytest.mark.parametrize("lens,H,Hkv,D", [((1100, 3, 200), 16, 16, 128), ((700, 650), 20, 20, 96), ((1600, 40), 12, 12, 64)])
+@pytest.mark.parametrize("kw", [dict(), dict(n_swa=300, softcap=8.0), dict(images=True)], ids=str)
+def test_f32_longer_prompts(pa, lens, H, Hkv, D, kw):
+    """Calls whose last row blocks are their critical path: 8 waves that share rows."""
+    one(pa, lens, H, Hkv, D, kind="f32", ends=image_ends if kw.get("images") else None,
+        **{k: v for k, v in kw.items() if k != "images"})
+
+
+@pytest.mark.parametrize("D,kind", [(80, "bf16"), (256, "f16"), (256, "f32")])
+def test_hidden_values_of_many_prompts(pa, D, kind):
+    """As below, with row blocks of every kind of workgroup: each prompt's last token holds NaN and infinities, which the
+    tokens before it do not see."""
+    g = torch.Generator().manual_seed(9)
+    T = sum(MANY)
+    q, k, v = rows(g, T, 16, 8, D, D, kind)
+    qsl = torch.tensor(np.concatenate([[0], np.cumsum(MANY)]), dtype=torch.int32, device="cuda")
+    prm = pa.PagedAttnParams(scale=D ** -0.5)
+    want = pa.prompt_attn(q, k, v, qsl, max(MANY), prm)
+    last = qsl[1:].long() - 1
+    keep = torch.ones(T, dtype=torch.bool, device="cuda")
+    keep[last] = False
+    for bad in (float("nan"), float("inf")):
+        k[last, :, 3] = bad
+        v[last, :, 5] = -bad
+        v[last, 0] = bad
+        assert torch.equal(pa.prompt_attn(q, k, v, qsl, max(MANY), prm)[keep], want[keep])
+
+
 @pytest.mark.parametrize("S,L", [(64, 30), (65, 30), (200, 9), (1500, 3), (5000, 1)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_prompt_counts(pa, S, L, causal):
