@@ -964,6 +964,9 @@ inline int64_t prompt_blocks(const PromptParams &p, int rows) {
     return std::min(all / rows + p.S, per * p.S) * p.Hkv;
 }
 
+// All prompts of at most 64 tokens, two tiles.
+inline bool prompt_short(const PromptParams &p) { return p.max_q <= 64 && p.T <= 64 * (int64_t) p.S; }
+
 template <int TY, int DK, int DV, bool VEC, int KW, int NW>
 static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
     const int64_t blocks = prompt_blocks(p, PromptShape<TY, DK, DV, VEC, KW, NW>::ROWS);
@@ -972,15 +975,19 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
 }
 
 // KW4, KW2: whether waves may share rows by four, by two (LDS holds their tiles).
-// They do in calls whose workgroups then still run at once: one of KW = 4 fits a
-// CU, two of KW = 2 (one 512-token prompt, H32/Hkv8/D128 bf16, 13 us, 20 with
-// KW = 1; one of 1024 23 and 33, and 48 with KW = 4).  Long causal prompts share by
-// two up to twice that (three times at head size 64): their last row blocks
-// see the most tokens and are the call's critical path (one of 2048 tokens 53
-// us, 59 with KW = 1, at H20/Hkv20/D96 32 and 46, one of 4096 at H14/Hkv2/D64 48
-// and 74; beyond, KW = 1: one of 2600, D128, 84 and 78; and for short prompts
-// or those that see all: 4 of 512 27 and 22, 2 images of 2048, D80, 73 and 62;
-// D256, H16/Hkv8: one of 2048 77 and 89, 4 of 1000 92 and 61).
+// They do in calls whose workgroups then still run at once, two on a CU (one at head
+// size 256): one 512-token prompt, H32/Hkv8/D128 bf16, 13 us, 17 with KW = 1, by
+// four at H14/Hkv2/D64 8, 9 with KW = 2 and 13 with KW = 1 (by four saves nothing
+// from head size 80 on).  Not up to 64 tokens, where joining costs more than the
+// second tile (one token 5.3 us, 6.0 with KW = 2; 16 prompts of 64 8 and 11).
+// Longer causal prompts share by two up to twice that (three times at head size
+// 64), since their last row blocks see the most tokens and are the call's critical
+// path, the less the more tokens there are beside them: with more than two such
+// prompts' up to 5/4 (twice).  Prompts of 900 and 300 tokens 20 us, 26 with KW = 1, one of
+// 2048 48 and 54, at H20/Hkv20/D96 31 and 46, one of 4096 at H14/Hkv2/D64 48 and 71, 4 of
+// 1000 19 and 23; slower beyond, for shorter ones and those that see all: one of
+// 2600, D128, 77 and 74, 3 of 600 26 and 21, 4 of 512 25 and 21, one that sees all of 2048
+// 83 and 73; D256, H16/Hkv8: one of 2048 70 and 90, 4 of 1000 89 and 56.
 //
 // NW8: whether workgroups have 8 waves (head size 256) where every CU then still
 // has one (4 prompts of 1000 tokens, H16/Hkv8, 57 us, 61 with 4 waves; 2 images of
@@ -988,13 +995,14 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
 template <int TY, int DK, int DV, bool KW4, bool KW2, bool NW8 = false>
 static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
     if (!vec) return launch_prompt_k<TY, DK, DV, false, 1, 4>(p, stream);
-    if constexpr (KW4)
-        if (prompt_blocks(p, 32) <= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 4, 4>(p, stream);
-    if constexpr (KW2) {
-        const int64_t at_once = (KW4 ? 2 : 1) * kPromptCus;
-        const bool critical = (p.causal || p.row_end) && p.max_q >= 1500;
-        if (prompt_blocks(p, 64) <= at_once * (!critical ? 1 : DK <= 64 ? 3 : 2))
-            return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
+    if (!prompt_short(p)) {
+        constexpr int at_once = (DK <= 128 ? 2 : 1) * kPromptCus;
+        const bool critical = (p.causal || p.row_end) && p.max_q >= 600, few = p.T <= 2 * (int64_t) p.max_q;
+        if constexpr (KW4)
+            if (prompt_blocks(p, 32) <= at_once) return launch_prompt_k<TY, DK, DV, true, 4, 4>(p, stream);
+        if constexpr (KW2)
+            if (prompt_blocks(p, 64) <= at_once * (!critical ? 4 : DK <= 64 ? few ? 12 : 8 : few ? 8 : 5) / 4)
+                return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
     }
     if constexpr (NW8)
         if (prompt_blocks(p, 256) >= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);

@@ -7,9 +7,9 @@ hipError_t launch_prompt_f16(const PromptParams &p, hipStream_t stream) {
     const bool vec = prompt_vec<1>(p);
     const int d = std::max(p.D, p.Dv);
     if (d <= 64) return launch_prompt_d<1, 64, 64, true, true>(p, vec, stream);
-    if (d <= 96 && p.D <= 80) return launch_prompt_d<1, 80, 96, true, true>(p, vec, stream);
-    if (d <= 96) return launch_prompt_d<1, 96, 96, true, true>(p, vec, stream);
-    if (d <= 128) return launch_prompt_d<1, 128, 128, true, true>(p, vec, stream);
+    if (d <= 96 && p.D <= 80) return launch_prompt_d<1, 80, 96, false, true>(p, vec, stream);
+    if (d <= 96) return launch_prompt_d<1, 96, 96, false, true>(p, vec, stream);
+    if (d <= 128) return launch_prompt_d<1, 128, 128, false, true>(p, vec, stream);
     return launch_prompt_d<1, 256, 256, false, true, true>(p, vec, stream);
 }
 

@@ -8,9 +8,9 @@ hipError_t launch_prompt_bf16(const PromptParams &p, hipStream_t stream) {
     const int d = std::max(p.D, p.Dv);
     if (d <= 64) return launch_prompt_d<30, 64, 64, true, true>(p, vec, stream);
     // (a fifth fewer products of Q and K than at 96: 6 images of 563 to 2100 tokens, H16/D80, 74 us, 76)
-    if (d <= 96 && p.D <= 80) return launch_prompt_d<30, 80, 96, true, true>(p, vec, stream);
-    if (d <= 96) return launch_prompt_d<30, 96, 96, true, true>(p, vec, stream);
-    if (d <= 128) return launch_prompt_d<30, 128, 128, true, true>(p, vec, stream);
+    if (d <= 96 && p.D <= 80) return launch_prompt_d<30, 80, 96, false, true>(p, vec, stream);
+    if (d <= 96) return launch_prompt_d<30, 96, 96, false, true>(p, vec, stream);
+    if (d <= 128) return launch_prompt_d<30, 128, 128, false, true>(p, vec, stream);
     return launch_prompt_d<30, 256, 256, false, true, true>(p, vec, stream);
 }
 

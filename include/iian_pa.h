@@ -325,8 +325,8 @@ int iian_pa_rope_kv_write(void *stream, const float *k_rows, const float *v_rows
  * memory.  *err_flag (when non-NULL) bit 3: a negative count or size, a grid
  * with h or w zero or a step below 1 (its tokens then count as none, its step
  * as 1), offsets out of order or outside [0, n_spans], or a position or end
- * past INT32_MAX, which is held there; seen in the runs that the step's tokens
- * need, those up to them.  At most 2^23 requests and 2^30 runs. */
+ * past INT32_MAX, which is held there; seen in the runs up to the step's
+ * tokens, and maybe in some behind them.  At most 2^23 requests and 2^30 runs. */
 int iian_pa_mrope_positions(void *stream, const int32_t *spans, const int32_t *span_off, int32_t n_spans,
                             const int32_t *num_computed, const int32_t *query_start_loc, int32_t n_seqs,
                             int32_t n_tokens, int32_t grid_full, int32_t *pos, int32_t *row_end, int32_t *err_flag);
