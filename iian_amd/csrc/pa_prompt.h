@@ -991,7 +991,8 @@ static hipError_t launch_prompt_k(const PromptParams &p, hipStream_t stream) {
 //
 // NW8: whether workgroups have 8 waves (head size 256) where every CU then still
 // has one (4 prompts of 1000 tokens, H16/Hkv8, 57 us, 61 with 4 waves; 2 images of
-// 2048 123 and 178; below, one causal prompt of 2048 95 and 89).
+// 2048 123 and 178; below, one causal prompt of 2048 95 and 89) and the longest prompt
+// has rows for more than 4 of them (64 prompts of 30 tokens 24 us, 21 with 4 waves).
 template <int TY, int DK, int DV, bool KW4, bool KW2, bool NW8 = false>
 static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t stream) {
     if (!vec) return launch_prompt_k<TY, DK, DV, false, 1, 4>(p, stream);
@@ -1005,7 +1006,8 @@ static hipError_t launch_prompt_d(const PromptParams &p, bool vec, hipStream_t s
                 return launch_prompt_k<TY, DK, DV, true, 2, 4>(p, stream);
     }
     if constexpr (NW8)
-        if (prompt_blocks(p, 256) >= kPromptCus) return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
+        if (prompt_blocks(p, 256) >= kPromptCus && (int64_t) p.max_q * p.gqa > 128)
+            return launch_prompt_k<TY, DK, DV, true, 1, 8>(p, stream);
     return launch_prompt_k<TY, DK, DV, true, 1, 4>(p, stream);
 }
 
